@@ -36,6 +36,8 @@ def _sources():
     units.append(("utility_ops", "utility_ops.cu", []))
     units.append(("sort_ops", "sort_ops.cu", []))
     units.append(("special_transforms", "special_transforms.cu", []))
+    for name in ("layer_norm", "token_log_probs", "embedding", "global_norm"):
+        units.append((name, name + ".cu", []))
     units.append(("device_env", "device_env.cu", []))
     units.append(("comm", "comm.cu", []))
     units.append(("runtime", "runtime.cu", []))

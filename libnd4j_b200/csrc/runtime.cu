@@ -1,5 +1,6 @@
 // Host-side runtime: error capture and the per-stream scratch workspace.
 #include "runtime.h"
+#include "entry_checks.h"
 #include <cstring>
 #include <map>
 #include <mutex>
@@ -110,8 +111,42 @@ Status staged_upload(cudaStream_t stream, void *dev, const void *host, size_t by
     return staging_commit(stream, slot, dev, bytes);
 }
 
+namespace {
+std::map<int, cudaMemPool_t> g_pools;      // one scratch pool per device
+}  // namespace
+
+Status Scratch::alloc(size_t bytes) {
+    int device = 0;
+    ND_CUDA(cudaGetDevice(&device));
+    cudaMemPool_t pool = nullptr;
+    {
+        std::lock_guard<std::mutex> lock(g_mu);
+        auto it = g_pools.find(device);
+        if (it == g_pools.end()) {
+            // making the pool touches no stream: it is allowed while this thread captures one
+            cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+            ND_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
+            cudaMemPoolProps props = {};
+            props.allocType = cudaMemAllocationTypePinned;
+            props.handleTypes = cudaMemHandleTypeNone;
+            props.location.type = cudaMemLocationTypeDevice;
+            props.location.id = device;
+            cudaError_t e = cudaMemPoolCreate(&pool, &props);
+            unsigned long long keep = ~0ull;
+            if (e == cudaSuccess) e = cudaMemPoolSetAttribute(pool, cudaMemPoolAttrReleaseThreshold, &keep);
+            const cudaError_t back = cudaThreadExchangeStreamCaptureMode(&mode);
+            if (e != cudaSuccess) return cuda_fail(e, "cudaMemPoolCreate(scratch)");
+            ND_CUDA(back);
+            g_pools[device] = pool;
+        } else pool = it->second;
+    }
+    ND_CUDA(cudaMallocFromPoolAsync(&ptr, bytes, pool, stream));
+    return kOk;
+}
+
 void release_workspaces() {
     std::lock_guard<std::mutex> lock(g_mu);
+    for (auto &kv : g_pools) cudaMemPoolTrimTo(kv.second, 0);
     for (auto &kv : g_blocks) {
         if (kv.second.dev) cudaFree(kv.second.dev);
         if (kv.second.host) cudaFreeHost(kv.second.host);
