@@ -14,9 +14,9 @@
 // in float (double for double data) and rounded once, after scaling and, where asked for, adding what grad holds.
 //
 // The sort is a least-significant-digit radix sort with digits of up to 9 bits: two passes up to a table of 2^18 rows.
-// Up to 65536 tokens one cluster of CTAs does all passes in one launch, the counts travelling through distributed
-// shared memory; the other CTAs of that launch write the zeros of the table meanwhile. Longer lists take three launches
-// per pass.
+// Up to 65536 tokens one cluster of CTAs does all passes in one launch, the counts and the keys travelling through
+// distributed shared memory; the other CTAs of that launch write the zeros of the table meanwhile. Longer lists take
+// three launches per pass.
 #include "../../include/nd4j_b200.h"
 #include <cooperative_groups.h>
 #include "device_utils.cuh"
@@ -28,17 +28,17 @@ namespace nd4jb200 {
 namespace {
 
 // ---- the order of the tokens -------------------------------------------------------------------------------------
-constexpr int kOrdThreads = 1024;
+constexpr int kOrdThreads = 512;
 constexpr int kOrdWarps = kOrdThreads / 32;
-constexpr int kOrdKeys = 8;                                   // per thread
-constexpr int kOrdTile = kOrdThreads * kOrdKeys;
+constexpr int kOrdMaxKeys = 16;                               // per thread
 constexpr int kOrdBits = 9;
-constexpr int kOrdBins = 1 << kOrdBits;
+constexpr int kOrdBins = 1 << kOrdBits;                       // one per thread
 constexpr int kOrdCluster = 8;
+static_assert(kOrdBins == kOrdThreads, "thread d looks after digit d");
 
 struct OrderArgs {
     const LL *tokens;
-    unsigned *key[2], *pos[2];       // ping-pong; `result` says which pair holds the sorted list
+    unsigned *key[2], *pos[2];       // ping-pong lists; one launch: the sorted list goes to the first
     unsigned n;
     unsigned vocab;                  // key of a token that takes no part: sorts behind all others
     int bits;                        // per digit
@@ -56,28 +56,14 @@ struct OrderArgs {
 struct OrderShared {
     unsigned short count[kOrdWarps][kOrdBins];   // per warp and digit: keys so far, then the tile-local start
     unsigned total[kOrdBins];                    // the tile's keys per digit (read by the other CTAs of a cluster)
-    unsigned base[kOrdBins];                     // where the tile's first key of the digit goes, less its local start
+    unsigned base[kOrdBins];                     // where the tile's first key of the digit goes
     unsigned warpSums[kOrdWarps];
 };
 
 ND_D unsigned order_key(const OrderArgs &a, LL token) { return token >= 0 && token < (LL) a.vocab ? (unsigned) token : a.vocab; }
 
-// Warp w holds the tile's keys [w * 256, w * 256 + 256), round r of it the next 32: "earlier" is (warp, round, lane).
-ND_D unsigned order_index(unsigned tile, int r) {
-    return tile * kOrdTile + (threadIdx.x >> 5) * (32 * kOrdKeys) + r * 32 + (threadIdx.x & 31);
-}
-ND_D void order_read(const OrderArgs &a, int pass, unsigned tile, unsigned (&key)[kOrdKeys], unsigned (&pos)[kOrdKeys]) {
-#pragma unroll
-    for (int r = 0; r < kOrdKeys; r++) {
-        const unsigned i = order_index(tile, r);
-        key[r] = pos[r] = 0;
-        if (i < a.n) {
-            if (pass == 0) { key[r] = order_key(a, a.tokens[i]); pos[r] = i; }
-            // written by other SMs in the pass before: from L2, where they meet
-            else { key[r] = __ldcg(a.key[(pass - 1) & 1] + i); pos[r] = __ldcg(a.pos[(pass - 1) & 1] + i); }
-        }
-    }
-}
+// Warp w holds keys [w * 32 * KPT, ...) of the tile, round r of it the next 32: "earlier" is (warp, round, lane).
+template <int KPT> ND_D unsigned order_local(int r) { return (threadIdx.x >> 5) * (32 * KPT) + r * 32 + (threadIdx.x & 31); }
 
 // Exclusive prefix sum over the CTA's threads.
 ND_D unsigned order_scan(unsigned v, unsigned *warpSums) {
@@ -90,64 +76,51 @@ ND_D unsigned order_scan(unsigned v, unsigned *warpSums) {
     }
     if (lane == 31) warpSums[warp] = inc;
     __syncthreads();
-    unsigned w = warpSums[lane], before = w;
+    unsigned before = 0;
 #pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-        const unsigned t = __shfl_up_sync(0xffffffffu, before, off);
-        if (lane >= off) before += t;
-    }
-    before = __shfl_sync(0xffffffffu, before - w, warp);
+    for (int w = 0; w < kOrdWarps; w++) before += w < warp ? warpSums[w] : 0u;
     __syncthreads();
     return before + inc - v;
 }
 
-// Rank of every key among the warp's earlier keys of its digit, and the tile's counts. Afterwards count[w][d] is the
-// number of the tile's keys of digit d in the warps before w, total[d] that of the tile.
-ND_D void order_rank(const OrderArgs &a, int pass, unsigned tile, const unsigned (&key)[kOrdKeys], unsigned (&rank)[kOrdKeys],
-                     OrderShared &s) {
+// Rank of every key among the warp's earlier keys of its digit, and the tile's counts; `live` of the tile's keys exist.
+// The lanes that share a digit are found with one ballot per bit of it (match.any takes a step per distinct value: a
+// tile of 4096 keys took 14 us per pass with it). Afterwards count[w][d] is the number of the tile's keys of digit d in
+// the warps before w, total[d] that of the tile.
+template <int KPT>
+ND_D void order_rank(const unsigned (&key)[KPT], unsigned (&rank)[KPT], int shift, int bits, unsigned live, OrderShared &s) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    unsigned *words = reinterpret_cast<unsigned *>(&s.count[0][0]);
-    for (int i = threadIdx.x; i < kOrdWarps * kOrdBins / 2; i += kOrdThreads) words[i] = 0;
-    __syncthreads();
+    uint4 *words = reinterpret_cast<uint4 *>(&s.count[0][0]);
 #pragma unroll
-    for (int r = 0; r < kOrdKeys; r++) {
-        const bool valid = order_index(tile, r) < a.n;
-        const unsigned d = valid ? (key[r] >> (pass * a.bits)) & ((1u << a.bits) - 1u) : 0xffffffffu;
-        const unsigned peers = __match_any_sync(0xffffffffu, d);
-        const unsigned earlier = __popc(peers & ((1u << lane) - 1u));
-        unsigned before = 0;
-        if (valid) before = s.count[warp][d];
+    for (int i = 0; i < kOrdWarps * kOrdBins / 8 / kOrdThreads; i++) words[i * kOrdThreads + threadIdx.x] = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+    const unsigned below = (1u << lane) - 1u, mask = (1u << bits) - 1u;
+#pragma unroll
+    for (int r = 0; r < KPT; r++) {
+        const bool valid = order_local<KPT>(r) < live;
+        const unsigned d = (key[r] >> shift) & mask;
+        unsigned peers = __ballot_sync(0xffffffffu, valid);
+#pragma unroll
+        for (int b = 0; b < kOrdBits; b++) {                  // bits beyond `bits` are 0 in every lane
+            const bool bit = (d >> b) & 1u;
+            const unsigned has = __ballot_sync(0xffffffffu, bit);
+            peers &= bit ? has : ~has;
+        }
+        const unsigned earlier = __popc(peers & below);
+        const unsigned before = s.count[warp][d];
         __syncwarp();
         if (valid && earlier == 0) s.count[warp][d] = (unsigned short) (before + __popc(peers));
         __syncwarp();
         rank[r] = before + earlier;
     }
     __syncthreads();
-    if (threadIdx.x < kOrdBins) {
-        unsigned run = 0;
-#pragma unroll 8
-        for (int w = 0; w < kOrdWarps; w++) {
-            const unsigned c = s.count[w][threadIdx.x];
-            s.count[w][threadIdx.x] = (unsigned short) run;
-            run += c;
-        }
-        s.total[threadIdx.x] = run;
-    }
-    __syncthreads();
-}
-
-ND_D void order_write(const OrderArgs &a, int pass, unsigned tile, const unsigned (&key)[kOrdKeys], const unsigned (&pos)[kOrdKeys],
-                      const unsigned (&rank)[kOrdKeys], const OrderShared &s) {
-    const int warp = threadIdx.x >> 5;
+    unsigned c[kOrdWarps], run = 0;
 #pragma unroll
-    for (int r = 0; r < kOrdKeys; r++) {
-        if (order_index(tile, r) < a.n) {
-            const unsigned d = (key[r] >> (pass * a.bits)) & ((1u << a.bits) - 1u);
-            const unsigned to = s.base[d] + s.count[warp][d] + rank[r];
-            __stcg(a.key[pass & 1] + to, key[r]);
-            __stcg(a.pos[pass & 1] + to, pos[r]);
-        }
-    }
+    for (int w = 0; w < kOrdWarps; w++) c[w] = s.count[w][threadIdx.x];
+#pragma unroll
+    for (int w = 0; w < kOrdWarps; w++) { s.count[w][threadIdx.x] = (unsigned short) run; run += c[w]; }
+    s.total[threadIdx.x] = run;
+    __syncthreads();
 }
 
 // One element of T that is zero in every type.
@@ -156,7 +129,12 @@ template <class T> ND_D void zero_rows(const OrderArgs &a, LL first, LL step) {
     if (a.zeroWords > 0 && a.zeroRow == a.cols) {              // one run
         const LL words = a.zeroRows * a.zeroWords;
         uint4 *p = reinterpret_cast<uint4 *>(z);
-        for (LL i = first; i < words; i += step) __stcs(p + i, make_uint4(0, 0, 0, 0));
+        LL i = first;
+        for (; i + 3 * step < words; i += 4 * step) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) __stcs(p + i + j * step, make_uint4(0, 0, 0, 0));
+        }
+        for (; i < words; i += step) __stcs(p + i, make_uint4(0, 0, 0, 0));
         return;
     }
     const LL perRow = a.zeroWords > 0 ? a.zeroWords : a.cols;
@@ -167,46 +145,86 @@ template <class T> ND_D void zero_rows(const OrderArgs &a, LL first, LL step) {
     }
 }
 
-// All passes in one launch. The first `sortCtas` CTAs (one cluster) sort a tile each, the others zero the table.
-template <class T>
+// All passes in one launch. The first `sortCtas` CTAs (one cluster) sort a tile of kOrdThreads * KPT keys each, the
+// others zero the table. Between the passes keys and positions go straight into the shared memory of the CTA whose tile
+// they belong to next: every CTA has its keys in registers when the totals have been exchanged, so one buffer serves.
+template <class T, int KPT>
 __global__ void __launch_bounds__(kOrdThreads) k_order_cluster(const OrderArgs a) {
     grid_dependency_sync();
-    __shared__ OrderShared s;
+    extern __shared__ unsigned ord_smem[];                    // keys, then positions, of the tile
+    __shared__ __align__(16) OrderShared s;
+    constexpr unsigned TILE = kOrdThreads * KPT;
     if (blockIdx.x >= (unsigned) a.sortCtas) {
         if (a.zero) zero_rows<T>(a, (LL) (blockIdx.x - a.sortCtas) * kOrdThreads + threadIdx.x, (LL) (gridDim.x - a.sortCtas) * kOrdThreads);
         return;
     }
     cg::cluster_group cl = cg::this_cluster();
     const unsigned tile = blockIdx.x, ctas = (unsigned) a.sortCtas;
+    const unsigned live = a.n > tile * TILE ? a.n - tile * TILE : 0u;      // of this tile's keys: all are in front
+    unsigned key[KPT], pos[KPT], rank[KPT];
+#pragma unroll
+    for (int r = 0; r < KPT; r++) {
+        const unsigned i = tile * TILE + order_local<KPT>(r);
+        key[r] = i < a.n ? order_key(a, a.tokens[i]) : 0u;
+        pos[r] = i;
+    }
     for (int pass = 0; pass < a.passes; pass++) {
-        unsigned key[kOrdKeys], pos[kOrdKeys], rank[kOrdKeys];
-        order_read(a, pass, tile, key, pos);
-        order_rank(a, pass, tile, key, rank, s);
-        cl.sync();                                            // every CTA's totals stand
+        const int shift = pass * a.bits;
+        order_rank<KPT>(key, rank, shift, a.bits, live, s);
+        cl.sync();                                            // every CTA's totals stand, every CTA has read its keys
         unsigned before = 0, all = 0;
-        if (threadIdx.x < kOrdBins) {
-            for (unsigned q = 0; q < ctas; q++) {
-                const unsigned c = cl.map_shared_rank(s.total, q)[threadIdx.x];
-                if (q < tile) before += c;
-                all += c;
+#pragma unroll 8
+        for (unsigned q = 0; q < ctas; q++) {
+            const unsigned c = cl.map_shared_rank(s.total, q)[threadIdx.x];
+            before += q < tile ? c : 0u;
+            all += c;
+        }
+        s.base[threadIdx.x] = order_scan(all, s.warpSums) + before;
+        __syncthreads();
+        const bool last = pass + 1 == a.passes;
+#pragma unroll
+        for (int r = 0; r < KPT; r++) {
+            if (order_local<KPT>(r) < live) {
+                const unsigned d = (key[r] >> shift) & ((1u << a.bits) - 1u);
+                const unsigned to = s.base[d] + s.count[threadIdx.x >> 5][d] + rank[r];
+                if (last) { a.key[0][to] = key[r]; a.pos[0][to] = pos[r]; }
+                else {
+                    unsigned *there = cl.map_shared_rank(ord_smem, to / TILE);
+                    there[to % TILE] = key[r];
+                    there[TILE + to % TILE] = pos[r];
+                }
             }
         }
-        const unsigned start = order_scan(all, s.warpSums);
-        if (threadIdx.x < kOrdBins) s.base[threadIdx.x] = start + before;
-        __syncthreads();
-        order_write(a, pass, tile, key, pos, rank, s);
-        cl.sync();                                            // keys written, and nobody reads the totals any more
+        cl.sync();                                            // keys stand, and nobody reads the totals any more
+        if (!last) {
+#pragma unroll
+            for (int r = 0; r < KPT; r++) { key[r] = ord_smem[order_local<KPT>(r)]; pos[r] = ord_smem[TILE + order_local<KPT>(r)]; }
+        }
+    }
+}
+
+template <int KPT> ND_D void order_read(const OrderArgs &a, int pass, unsigned tile, unsigned (&key)[KPT], unsigned (&pos)[KPT]) {
+    const unsigned *fromKey = a.key[(pass - 1) & 1], *fromPos = a.pos[(pass - 1) & 1];
+#pragma unroll
+    for (int r = 0; r < KPT; r++) {
+        const unsigned i = tile * (kOrdThreads * KPT) + order_local<KPT>(r);
+        key[r] = pos[r] = 0;
+        if (i < a.n) {
+            key[r] = pass == 0 ? order_key(a, a.tokens[i]) : fromKey[i];
+            pos[r] = pass == 0 ? i : fromPos[i];
+        }
     }
 }
 
 __global__ void __launch_bounds__(kOrdThreads) k_order_count(const OrderArgs a, int pass) {
     grid_dependency_sync();
-    __shared__ OrderShared s;
+    __shared__ __align__(16) OrderShared s;
+    constexpr unsigned TILE = kOrdThreads * kOrdMaxKeys;
     for (unsigned tile = blockIdx.x; tile < a.tiles; tile += gridDim.x) {
-        unsigned key[kOrdKeys], pos[kOrdKeys], rank[kOrdKeys];
-        order_read(a, pass, tile, key, pos);
-        order_rank(a, pass, tile, key, rank, s);
-        if (threadIdx.x < kOrdBins) a.hist[(LL) tile * kOrdBins + threadIdx.x] = s.total[threadIdx.x];
+        unsigned key[kOrdMaxKeys], pos[kOrdMaxKeys], rank[kOrdMaxKeys];
+        order_read<kOrdMaxKeys>(a, pass, tile, key, pos);
+        order_rank<kOrdMaxKeys>(key, rank, pass * a.bits, a.bits, a.n - tile * TILE, s);
+        a.hist[(LL) tile * kOrdBins + threadIdx.x] = s.total[threadIdx.x];
         __syncthreads();
     }
 }
@@ -216,29 +234,45 @@ __global__ void __launch_bounds__(kOrdThreads) k_order_starts(const OrderArgs a)
     grid_dependency_sync();
     __shared__ unsigned warpSums[kOrdWarps];
     unsigned run = 0;
-    const bool live = threadIdx.x < kOrdBins;
-    if (live) for (unsigned t = 0; t < a.tiles; t++) run += a.hist[(LL) t * kOrdBins + threadIdx.x];
-    unsigned at = order_scan(live ? run : 0, warpSums);
-    if (live) {
-        for (unsigned t = 0; t < a.tiles; t++) {
-            unsigned &h = a.hist[(LL) t * kOrdBins + threadIdx.x];
-            const unsigned c = h;
-            h = at;
-            at += c;
-        }
+#pragma unroll 8
+    for (unsigned t = 0; t < a.tiles; t++) run += a.hist[(LL) t * kOrdBins + threadIdx.x];
+    unsigned at = order_scan(run, warpSums);
+    unsigned t = 0;
+    for (; t + 8 <= a.tiles; t += 8) {
+        unsigned c[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) c[k] = a.hist[(LL) (t + k) * kOrdBins + threadIdx.x];
+#pragma unroll
+        for (int k = 0; k < 8; k++) { a.hist[(LL) (t + k) * kOrdBins + threadIdx.x] = at; at += c[k]; }
+    }
+    for (; t < a.tiles; t++) {
+        const unsigned c = a.hist[(LL) t * kOrdBins + threadIdx.x];
+        a.hist[(LL) t * kOrdBins + threadIdx.x] = at;
+        at += c;
     }
 }
 
 __global__ void __launch_bounds__(kOrdThreads) k_order_scatter(const OrderArgs a, int pass) {
     grid_dependency_sync();
-    __shared__ OrderShared s;
+    __shared__ __align__(16) OrderShared s;
+    constexpr unsigned TILE = kOrdThreads * kOrdMaxKeys;
+    unsigned *toKey = a.key[pass & 1], *toPos = a.pos[pass & 1];
     for (unsigned tile = blockIdx.x; tile < a.tiles; tile += gridDim.x) {
-        unsigned key[kOrdKeys], pos[kOrdKeys], rank[kOrdKeys];
-        order_read(a, pass, tile, key, pos);
-        order_rank(a, pass, tile, key, rank, s);
-        if (threadIdx.x < kOrdBins) s.base[threadIdx.x] = a.hist[(LL) tile * kOrdBins + threadIdx.x];
+        unsigned key[kOrdMaxKeys], pos[kOrdMaxKeys], rank[kOrdMaxKeys];
+        const unsigned live = a.n - tile * TILE;
+        order_read<kOrdMaxKeys>(a, pass, tile, key, pos);
+        order_rank<kOrdMaxKeys>(key, rank, pass * a.bits, a.bits, live, s);
+        s.base[threadIdx.x] = a.hist[(LL) tile * kOrdBins + threadIdx.x];
         __syncthreads();
-        order_write(a, pass, tile, key, pos, rank, s);
+#pragma unroll
+        for (int r = 0; r < kOrdMaxKeys; r++) {
+            if (order_local<kOrdMaxKeys>(r) < live) {
+                const unsigned d = (key[r] >> (pass * a.bits)) & ((1u << a.bits) - 1u);
+                const unsigned to = s.base[d] + s.count[threadIdx.x >> 5][d] + rank[r];
+                toKey[to] = key[r];
+                toPos[to] = pos[r];
+            }
+        }
         __syncthreads();
     }
 }
@@ -283,7 +317,7 @@ template <class T, int V> struct EmbRun {
 template <class T, int V> struct alignas(V == 1 ? sizeof(T) : 16) EmbWord : EmbRun<T, V> {};
 
 template <class T, int V>
-__global__ void __launch_bounds__(kEmbThreads) k_embedding(const EmbArgs a) {
+__global__ void __launch_bounds__(kEmbThreads, 6) k_embedding(const EmbArgs a) {
     grid_dependency_sync();
     typedef typename Elem<T>::C C;
     const int groups = kEmbThreads / a.group, g = threadIdx.x / a.group, t = threadIdx.x - g * a.group;
@@ -291,23 +325,26 @@ __global__ void __launch_bounds__(kEmbThreads) k_embedding(const EmbArgs a) {
     T *z = static_cast<T *>(a.dst);
     const C scale = (C) a.scale;
     for (LL i0 = ((LL) blockIdx.x * groups + g) * kEmbRows; i0 < a.n; i0 += (LL) gridDim.x * groups * kEmbRows) {
-        LL token[kEmbRows];
+        int row[kEmbRows];
+        bool in[kEmbRows];
+        C other[kEmbRows];
 #pragma unroll
-        for (int r = 0; r < kEmbRows; r++) token[r] = i0 + r < a.n ? a.tokens[i0 + r] : -1;
+        for (int r = 0; r < kEmbRows; r++) {
+            const LL token = i0 + r < a.n ? a.tokens[i0 + r] : -1;
+            in[r] = token >= 0 && token < a.vocab;
+            row[r] = in[r] ? (int) token : 0;
+            other[r] = token < 0 ? C(0) : (C) NAN;
+        }
         for (int w = t; w < a.words; w += a.group) {
             EmbWord<T, V> v[kEmbRows];
 #pragma unroll
             for (int r = 0; r < kEmbRows; r++)
-                if (token[r] >= 0 && token[r] < a.vocab) v[r].load(table + token[r] * a.srcRow + (LL) w * V * a.srcCol);
+                if (in[r]) v[r].load(table + row[r] * a.srcRow + (LL) w * V * a.srcCol);
 #pragma unroll
             for (int r = 0; r < kEmbRows; r++) {
                 if (i0 + r >= a.n) break;
 #pragma unroll
-                for (int k = 0; k < V; k++) {
-                    if (token[r] < 0) v[r].v[k] = Elem<T>::from_c(C(0));
-                    else if (token[r] >= a.vocab) v[r].v[k] = Elem<T>::from_c((C) NAN);
-                    else v[r].v[k] = Elem<T>::from_c(Elem<T>::to_c(v[r].v[k]) * scale);
-                }
+                for (int k = 0; k < V; k++) v[r].v[k] = Elem<T>::from_c(in[r] ? Elem<T>::to_c(v[r].v[k]) * scale : other[r]);
                 v[r].store(z + (i0 + r) * a.dstRow + (LL) w * V * a.dstCol);
             }
         }
@@ -332,46 +369,49 @@ template <int V, class C> ND_D void emb_partial(const EmbArgs &a, unsigned chunk
     for (int k = 0; k < V; k++) p[k] = sum[k];
 }
 
-// A group of threads walks a chunk of the sorted list, each thread one run of V columns. Four rows are in flight.
+// A group of threads walks a chunk of the sorted list, each thread one run of V columns. The chunk's keys and positions
+// are fetched first, so that the rows themselves can be read without waiting for one another, eight at a time.
+constexpr int kEmbMaxChunk = 64;
 template <class T, int V>
-__global__ void __launch_bounds__(kEmbThreads) k_embedding_sums(const EmbArgs a) {
+__global__ void __launch_bounds__(kEmbThreads, 4) k_embedding_sums(const EmbArgs a) {
     grid_dependency_sync();
     typedef typename Elem<T>::C C;
+    constexpr int R = 8;
+    extern __shared__ unsigned emb_smem[];                      // per group: keys of one entry before .. one behind, positions
     const int groups = kEmbThreads / a.group, g = threadIdx.x / a.group, t = threadIdx.x - g * a.group;
-    const unsigned chunk = blockIdx.x * groups + g;
+    const unsigned chunk = blockIdx.x * groups + g, n = (unsigned) a.n, vocab = (unsigned) a.vocab;
+    unsigned *key = emb_smem + g * (2 * kEmbMaxChunk + 2) + 1, *pos = key + kEmbMaxChunk + 1;
+    const unsigned first = chunk < a.chunks ? chunk * a.chunk : n;
+    const int len = n - first < a.chunk ? (int) (n - first) : (int) a.chunk;
+    for (int i = t - 1; i <= len; i += a.group) {
+        const bool in = i < 0 ? first > 0 : first + i < n;
+        key[i] = in ? a.key[first + i] : (i < 0 ? 0xffffffffu : vocab);        // no token has these
+        if (i >= 0 && i < len) pos[i] = a.pos[first + i];
+    }
+    __syncthreads();
     const T *dz = static_cast<const T *>(a.src);
-    if (chunk >= a.chunks) return;
-    const unsigned n = (unsigned) a.n, vocab = (unsigned) a.vocab;
-    const unsigned first = chunk * a.chunk, last = n - first < a.chunk ? n : first + a.chunk;
-    const unsigned before = first > 0 ? a.key[first - 1] : 0xffffffffu;      // no key: vocab is below 2^31
     for (int w = t + (int) blockIdx.y * a.group; w < a.words; w += a.group * (int) gridDim.y) {
         C sum[V];
 #pragma unroll
         for (int k = 0; k < V; k++) sum[k] = C(0);
-        unsigned key = a.key[first];
-        bool head = key == before;                              // the run began in an earlier chunk
-        for (unsigned i = first; i < last && key < vocab; i += 4) {
-            EmbWord<T, V> v[4];
-            unsigned next[4];
+        bool head = key[0] == key[-1];                          // the run began in an earlier chunk
+        for (int i = 0; i < len && key[i] < vocab; i += R) {
+            EmbWord<T, V> v[R];
 #pragma unroll
-            for (int q = 0; q < 4; q++) {
-                if (i + q < last) {
-                    if (a.key[i + q] < vocab) v[q].load(dz + (LL) a.pos[i + q] * a.srcRow + (LL) w * V * a.srcCol);
-                    next[q] = i + q + 1 < n ? a.key[i + q + 1] : vocab;
-                }
-            }
+            for (int q = 0; q < R; q++)
+                if (i + q < len && key[i + q] < vocab) v[q].load(dz + (LL) pos[i + q] * a.srcRow + (LL) w * V * a.srcCol);
 #pragma unroll
-            for (int q = 0; q < 4; q++) {
-                if (i + q >= last || key >= vocab) break;
+            for (int q = 0; q < R; q++) {
+                if (i + q >= len || key[i + q] >= vocab) break;
 #pragma unroll
                 for (int k = 0; k < V; k++) sum[k] += Elem<T>::to_c(v[q].v[k]);
-                if (next[q] != key || i + q + 1 == last) {
+                const bool ends = key[i + q + 1] != key[i + q];
+                if (ends || i + q + 1 == len) {
                     // the run ends here, or the chunk does
                     if (head) emb_partial<V>(a, chunk, 0, w, sum);
-                    else if (next[q] != key) emb_finish<T, V>(a, key, w, sum);
+                    else if (ends) emb_finish<T, V>(a, key[i + q], w, sum);
                     else emb_partial<V>(a, chunk, 1, w, sum);
                     head = false;
-                    key = next[q];
 #pragma unroll
                     for (int k = 0; k < V; k++) sum[k] = C(0);
                 }
@@ -381,42 +421,61 @@ __global__ void __launch_bounds__(kEmbThreads) k_embedding_sums(const EmbArgs a)
 }
 
 // Runs that cross chunks: the CTA of the chunk that such a run begins in adds up the tail there and the heads of the
-// chunks it reaches, eight at a time, the eight sums in order.
+// chunks it reaches, eight at a time, the eight sums in order. Most chunks have no such run and their CTA ends at once.
 template <class T>
 __global__ void __launch_bounds__(256) k_embedding_join(const EmbArgs a) {
     grid_dependency_sync();
     typedef typename Elem<T>::C C;
-    __shared__ C part[8][32];
-    const unsigned chunk = blockIdx.x, n = (unsigned) a.n;
+    constexpr int W = 4;                                        // columns per lane
+    __shared__ C part[8][32 * W];
+    const unsigned chunk = blockIdx.x;
     const unsigned end = (chunk + 1) * a.chunk;                 // there is a next chunk: the grid leaves out the last one
-    const unsigned key = a.key[end - 1];
-    if (key >= (unsigned) a.vocab || a.key[end] != key) return;                                 // no run crosses
     const unsigned first = chunk * a.chunk;
-    if (first > 0 && a.key[first] == key && a.key[first - 1] == key) return;                    // began earlier
-    // the chunks the run reaches: up to the one that holds its last entry, found by bisection
-    unsigned lo = end, hi = n - 1;
-    while (lo < hi) {
-        const unsigned mid = lo + (hi - lo + 1) / 2;
-        if (a.key[mid] == key) lo = mid; else hi = mid - 1;
+    const unsigned key = a.key[end - 1], after = a.key[end], start = a.key[first], before = first > 0 ? a.key[first - 1] : 0xffffffffu;
+    if (key >= (unsigned) a.vocab || after != key) return;      // no run crosses
+    if (start == key && before == key) return;                  // it began earlier
+    // the chunks the run reaches are those that begin with its key: 256 of them are looked at in one step
+    unsigned reach = chunk;
+    for (;;) {
+        const LL q = (LL) reach + 1 + threadIdx.x;
+        const int more = __syncthreads_count(q < a.chunks && a.key[q * a.chunk] == key);
+        reach += more;
+        if (more < 256) break;
     }
-    const unsigned reach = lo / a.chunk;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const C *p = static_cast<const C *>(a.partials);
-    for (LL c0 = (LL) blockIdx.y * 32; c0 < a.cols; c0 += (LL) gridDim.y * 32) {
-        const LL c = c0 + lane;
-        C s = C(0);
-        if (c < a.cols) {
-            if (warp == 0) s = p[((LL) chunk * 2 + 1) * a.cols + c];
-            for (unsigned q = chunk + 1 + warp; q <= reach; q += 8) s += p[(LL) q * 2 * a.cols + c];
+    for (LL c0 = (LL) blockIdx.y * 32 * W; c0 < a.cols; c0 += (LL) gridDim.y * 32 * W) {
+        C s[W];
+#pragma unroll
+        for (int k = 0; k < W; k++) s[k] = C(0);
+        if (warp == 0) {
+#pragma unroll
+            for (int k = 0; k < W; k++) if (c0 + k * 32 + lane < a.cols) s[k] = p[((LL) chunk * 2 + 1) * a.cols + c0 + k * 32 + lane];
+        }
+        for (unsigned q = chunk + 1 + warp; q <= reach; q += 32) {          // four of the warp's chunks in flight
+            C v[4][W];
+#pragma unroll
+            for (int u = 0; u < 4; u++)
+#pragma unroll
+                for (int k = 0; k < W; k++)
+                    v[u][k] = q + 8 * u <= reach && c0 + k * 32 + lane < a.cols ? p[(LL) (q + 8 * u) * 2 * a.cols + c0 + k * 32 + lane] : C(0);
+#pragma unroll
+            for (int u = 0; u < 4; u++)
+#pragma unroll
+                for (int k = 0; k < W; k++) s[k] += v[u][k];
         }
         __syncthreads();
-        part[warp][lane] = s;
+#pragma unroll
+        for (int k = 0; k < W; k++) part[warp][k * 32 + lane] = s[k];
         __syncthreads();
-        if (warp == 0 && c < a.cols) {
-            for (int q = 1; q < 8; q++) s += part[q][lane];
+        const LL c = c0 + threadIdx.x;
+        if (threadIdx.x < 32 * W && c < a.cols) {
+            C sum = part[0][threadIdx.x];
+#pragma unroll
+            for (int q = 1; q < 8; q++) sum += part[q][threadIdx.x];
             T *g = static_cast<T *>(a.dst) + (LL) key * a.dstRow + c * a.dstCol;
-            s *= (C) a.scale;
-            Elem<T>::store(g, a.accumulate ? Elem<T>::load(g) + s : s);
+            sum *= (C) a.scale;
+            Elem<T>::store(g, a.accumulate ? Elem<T>::load(g) + sum : sum);
         }
     }
 }
@@ -440,9 +499,11 @@ template <class T> Status emb_lookup(EmbArgs &a, bool words, cudaStream_t st) {
     return kOk;
 }
 
-template <class T> Status launch_order_cluster(const OrderArgs &o, unsigned grid, unsigned cluster, cudaStream_t st) {
+template <class T, int KPT> Status launch_order_cluster(const OrderArgs &o, unsigned grid, unsigned cluster, cudaStream_t st) {
+    const size_t smem = o.passes > 1 ? 2 * sizeof(unsigned) * kOrdThreads * KPT : 0;
+    ND_CUDA(cudaFuncSetAttribute(k_order_cluster<T, KPT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem));
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid); cfg.blockDim = dim3(kOrdThreads); cfg.stream = st;
+    cfg.gridDim = dim3(grid); cfg.blockDim = dim3(kOrdThreads); cfg.dynamicSmemBytes = smem; cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = cluster; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
@@ -450,7 +511,7 @@ template <class T> Status launch_order_cluster(const OrderArgs &o, unsigned grid
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = g_tuning[kTuneOverlapLaunch] ? 2 : 1;
-    cudaLaunchKernelEx(&cfg, k_order_cluster<T>, o);
+    cudaLaunchKernelEx(&cfg, k_order_cluster<T, KPT>, o);
     count_launch();
     return kOk;
 }
@@ -461,16 +522,28 @@ template <class T> Status order_tokens(OrderArgs &o, int *result, cudaStream_t s
     while (width < 32 && (o.vocab >> width) != 0) width++;               // keys go up to vocab itself
     o.passes = (int) ceil_div(width, kOrdBits);
     o.bits = (int) ceil_div(width, o.passes);
-    o.tiles = (unsigned) ceil_div(o.n, kOrdTile);
-    *result = (o.passes - 1) & 1;
-    const unsigned zeroCtas = o.zero ? (unsigned) kNumSMs : 0u;
-    if (o.tiles <= (unsigned) kOrdCluster) {
+    const unsigned zeroCtas = o.zero ? (unsigned) kNumSMs * 3 : 0u;
+    // One cluster, of as many CTAs as the tokens fill with the fewest keys per thread that let eight CTAs hold them
+    // all: the time goes with the keys per thread.
+    for (int kpt = 1; kpt <= kOrdMaxKeys; kpt *= 2) {
+        const LL tile = (LL) kOrdThreads * kpt;
+        if (o.n > tile * kOrdCluster) continue;
         unsigned cluster = 1;
-        while (cluster < o.tiles) cluster *= 2;
+        while (cluster * tile < o.n) cluster *= 2;
         o.sortCtas = (int) cluster;
-        return launch_order_cluster<T>(o, cluster + zeroCtas / cluster * cluster, cluster, st);
+        *result = 0;
+        const unsigned grid = cluster + zeroCtas / cluster * cluster;
+        switch (kpt) {
+            case 1: return launch_order_cluster<T, 1>(o, grid, cluster, st);
+            case 2: return launch_order_cluster<T, 2>(o, grid, cluster, st);
+            case 4: return launch_order_cluster<T, 4>(o, grid, cluster, st);
+            case 8: return launch_order_cluster<T, 8>(o, grid, cluster, st);
+            default: return launch_order_cluster<T, 16>(o, grid, cluster, st);
+        }
     }
-    if (o.zero) launch_kernel(k_zero_rows<T>, dim3(zeroCtas * 2), dim3(kOrdThreads), st, o);
+    *result = (o.passes - 1) & 1;
+    o.tiles = (unsigned) ceil_div(o.n, kOrdThreads * kOrdMaxKeys);
+    if (o.zero) launch_kernel(k_zero_rows<T>, dim3((unsigned) kNumSMs * 4), dim3(kOrdThreads), st, o);
     const unsigned grid = o.tiles < (unsigned) kNumSMs * 2 ? o.tiles : (unsigned) kNumSMs * 2;
     for (int pass = 0; pass < o.passes; pass++) {
         launch_kernel(k_order_count, dim3(grid), dim3(kOrdThreads), st, o, pass);
@@ -478,6 +551,19 @@ template <class T> Status order_tokens(OrderArgs &o, int *result, cudaStream_t s
         launch_kernel(k_order_scatter, dim3(grid), dim3(kOrdThreads), st, o, pass);
     }
     return kOk;
+}
+
+template <class T, int V> void launch_sums(const EmbArgs &a, dim3 grid, cudaStream_t st) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid; cfg.blockDim = dim3(kEmbThreads); cfg.stream = st;
+    cfg.dynamicSmemBytes = sizeof(unsigned) * (2 * kEmbMaxChunk + 2) * (kEmbThreads / a.group);
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = g_tuning[kTuneOverlapLaunch] ? 1 : 0;
+    cudaLaunchKernelEx(&cfg, k_embedding_sums<T, V>, a);
+    count_launch();
 }
 
 template <class T> Status emb_gradient(EmbArgs &a, OrderArgs &o, bool words, cudaStream_t st) {
@@ -492,13 +578,13 @@ template <class T> Status emb_gradient(EmbArgs &a, OrderArgs &o, bool words, cud
     a.group = group_for(a.words);
     const LL slices = ceil_div(a.words, a.group);
     // Longer chunks mean fewer partial sums, shorter ones more CTAs: the longest of 8 .. 64 that still gives every SM
-    // eight CTAs, as far as there are that many rows.
-    LL chunk = 64;
-    while (chunk > 8 && ceil_div(a.n, chunk) * slices * a.group / kEmbThreads < (LL) kNumSMs * 8) chunk /= 2;
+    // three CTAs, as far as there are that many rows.
+    LL chunk = kEmbMaxChunk;
+    while (chunk > 8 && ceil_div(a.n, chunk) * slices * a.group / kEmbThreads < (LL) kNumSMs * 3) chunk /= 2;
     a.chunk = (unsigned) chunk;
     a.chunks = (unsigned) ceil_div(a.n, chunk);
     const size_t list = round_up((size_t) a.n * sizeof(unsigned), 256);
-    const size_t hist = round_up((size_t) ceil_div(a.n, kOrdTile) * kOrdBins * sizeof(unsigned), 256);
+    const size_t hist = round_up((size_t) ceil_div(a.n, kOrdThreads * kOrdMaxKeys) * kOrdBins * sizeof(unsigned), 256);
     Scratch scratch(st);
     ND_TRY(scratch.alloc(4 * list + hist + (size_t) a.chunks * 2 * (size_t) a.cols * sizeof(C)));
     for (int k = 0; k < 2; k++) { o.key[k] = scratch.at<unsigned>(2 * k * list); o.pos[k] = scratch.at<unsigned>((2 * k + 1) * list); }
@@ -508,10 +594,10 @@ template <class T> Status emb_gradient(EmbArgs &a, OrderArgs &o, bool words, cud
     ND_TRY(order_tokens<T>(o, &result, st));
     a.key = o.key[result]; a.pos = o.pos[result];
     const dim3 grid((unsigned) ceil_div(a.chunks, kEmbThreads / a.group), (unsigned) (slices < 65535 ? slices : 65535));
-    if (words) launch_kernel(k_embedding_sums<T, V>, grid, dim3(kEmbThreads), st, a);
-    else launch_kernel(k_embedding_sums<T, 1>, grid, dim3(kEmbThreads), st, a);
+    if (words) launch_sums<T, V>(a, grid, st);
+    else launch_sums<T, 1>(a, grid, st);
     if (a.chunks > 1) {
-        const LL slabs = ceil_div(a.cols, 32);
+        const LL slabs = ceil_div(a.cols, 128);
         launch_kernel(k_embedding_join<T>, dim3(a.chunks - 1, (unsigned) (slabs < 64 ? slabs : 64)), dim3(256), st, a);
     }
     ND_CUDA(cudaGetLastError());

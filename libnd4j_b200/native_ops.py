@@ -15,6 +15,8 @@ is used as the CUDA stream, exactly as the reference does (blas/cuda/NativeOps.c
 """
 import ctypes
 import os
+import sys
+from array import array
 
 import numpy as np
 
@@ -23,9 +25,10 @@ LIB_PATH = os.path.join(_HERE, "libnd4jb200.so")
 
 FLOAT, DOUBLE, HALF = 0, 1, 2
 _SUFFIX = {"Float": FLOAT, "Double": DOUBLE, "Half": HALF}
-# element type of a call, and the type that sums and statistics have
-_KINDS = {FLOAT: "torch.float32", DOUBLE: "torch.float64", HALF: "torch.float16"}
-_WIDE = {FLOAT: "torch.float32", DOUBLE: "torch.float64", HALF: "torch.float32"}
+# names of the element type of a call, and of the type that sums and statistics have
+_KINDS = {FLOAT: "float32", DOUBLE: "float64", HALF: "float16"}
+_WIDE = {FLOAT: "float32", DOUBLE: "float64", HALF: "float32"}
+_torch_kinds = {}
 
 # copy directions of NativeOps::memcpy* (blas/cuda/NativeOps.cu:4038-4075)
 HOST_TO_HOST, HOST_TO_DEVICE, DEVICE_TO_HOST, DEVICE_TO_DEVICE = 0, 1, 2, 3
@@ -63,6 +66,16 @@ def _ints(a):
         return None, None
     arr = np.ascontiguousarray(a, dtype=np.int32)
     return arr, arr.ctypes.data_as(ctypes.POINTER(ctypes.c_int))
+
+
+def _descriptor(a):
+    """A shapeInfo (or another list of 64-bit integers) as the bytes that a C function reads, and as a list. (An array's
+    own address costs ctypes ten times as much.)"""
+    if a is None:
+        return None, None
+    if type(a) is not np.ndarray or a.dtype != np.int64:
+        a = np.asarray(a, dtype=np.int64)
+    return a.tobytes(), a.tolist()
 
 
 def load_library(path=None):
@@ -105,14 +118,14 @@ def load_library(path=None):
         "nd4jb200_exec_chain": (i, [vp, i, i, vp, llp, vp, llp, ip, i, i, vp, i, vp, llp, vp, vp, llp]),
         "nd4jb200_exec_meta_predicate_shape": (i, [vp, i, i, i, i, i, vp, llp, vp, llp, vp, llp, vp, vp, d, d]),
         "nd4jb200_exec_meta_predicate_strided": (i, [vp, i, i, i, i, i, ll, vp, ll, vp, ll, vp, ll, vp, vp, d, d]),
-        "nd4jb200_exec_layer_norm": (i, [vp, i, vp, llp, vp, vp, d, vp, llp, vp, vp, ip, i]),
-        "nd4jb200_exec_layer_norm_grad": (i, [vp, i, vp, llp, vp, vp, vp, vp, llp, vp, llp, vp, vp, ip, i]),
-        "nd4jb200_exec_token_log_probs": (i, [vp, i, vp, llp, vp, d, vp, vp, vp, vp, i, vp, vp]),
-        "nd4jb200_exec_token_log_probs_grad": (i, [vp, i, vp, llp, vp, d, vp, vp, vp, vp, vp, vp, llp]),
-        "nd4jb200_exec_embedding": (i, [vp, i, vp, llp, vp, d, vp, llp]),
-        "nd4jb200_exec_embedding_grad": (i, [vp, i, vp, d, vp, llp, vp, llp, i]),
-        "nd4jb200_exec_global_norm": (i, [vp, i, vp, llp, i, vp]),
-        "nd4jb200_exec_clip_by_global_norm": (i, [vp, i, vp, vp, llp, i, d, vp]),
+        "nd4jb200_exec_layer_norm": (i, [vp, i, vp, vp, vp, vp, d, vp, vp, vp, vp, vp, i]),
+        "nd4jb200_exec_layer_norm_grad": (i, [vp, i, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, i]),
+        "nd4jb200_exec_token_log_probs": (i, [vp, i, vp, vp, vp, d, vp, vp, vp, vp, i, vp, vp]),
+        "nd4jb200_exec_token_log_probs_grad": (i, [vp, i, vp, vp, vp, d, vp, vp, vp, vp, vp, vp, vp]),
+        "nd4jb200_exec_embedding": (i, [vp, i, vp, vp, vp, d, vp, vp]),
+        "nd4jb200_exec_embedding_grad": (i, [vp, i, vp, d, vp, vp, vp, vp, i]),
+        "nd4jb200_exec_global_norm": (i, [vp, i, vp, vp, i, vp]),
+        "nd4jb200_exec_clip_by_global_norm": (i, [vp, i, vp, vp, vp, i, d, vp]),
         "nd4jb200_comm_unique_id": (i, [vp]),
         "nd4jb200_comm_init": (i, [vp, i, i]),
         "nd4jb200_comm_destroy": (i, []),
@@ -370,34 +383,52 @@ class NativeOps:
                                                  _ptr(y), ysp, _ptr(pairwiseExtra), _ptr(z), zsp))
 
     # ---- between a language model's matrix products (no counterpart among the reference's members) ----
-    def _tensor(self, obj, name, kind=None, count=None):
-        """Pointer of a device array. What a torch tensor tells about itself is checked: the device, the element
+    # These are called once per token in the smallest use, so their checks are kept to what a few attribute reads tell.
+    @staticmethod
+    def _kinds(dt):
+        """torch's element types for a call: its own, the wide one, the one of tokens (None without torch)."""
+        if dt not in _torch_kinds:
+            torch = sys.modules.get("torch")
+            if torch is None or dt not in _KINDS:
+                return None, None, None
+            _torch_kinds[dt] = getattr(torch, _KINDS[dt]), getattr(torch, _WIDE[dt]), torch.int64
+        return _torch_kinds[dt]
+
+    def _tensor(self, obj, name, device, kind=None, count=None):
+        """Address of a device array. What a torch tensor tells about itself is checked: the device, the element
         type and, for arrays that have to be dense, that they are and hold `count` elements."""
-        if obj is None or not hasattr(obj, "is_cuda"):
+        if obj is None:
+            return None
+        try:
+            at = obj.get_device()
+        except AttributeError:
             return _ptr(obj)
-        if not obj.is_cuda:
-            raise Nd4jError(1, "%s is not in device memory" % name)
-        if obj.device.index != self.lib.nd4jb200_get_device():
-            raise Nd4jError(1, "%s lives on device %d, which is not the current one" % (name, obj.device.index))
-        if kind is not None and str(obj.dtype) != kind:
+        if at != device or at < 0:
+            raise Nd4jError(1, "%s is not in device memory" % name if at < 0 else
+                            "%s lives on device %d, which is not the current one" % (name, at))
+        if kind is not None and obj.dtype is not kind:
             raise Nd4jError(1, "%s holds %s, not %s" % (name, obj.dtype, kind))
         if count is not None and (obj.numel() != count or not obj.is_contiguous()):
             raise Nd4jError(1, "%s must be dense and hold %d elements" % (name, count))
         return obj.data_ptr()
 
-    def _array(self, obj, name, kind, info):
-        """Pointer of a device array that a shapeInfo describes: a torch tensor's storage has to reach as far."""
-        p = self._tensor(obj, name, kind)
-        if info is not None and hasattr(obj, "untyped_storage"):
-            r = int(info[0])
+    def _array(self, obj, name, device, kind, info):
+        """Address of a device array that a shapeInfo (a list here) describes: a torch tensor's memory has to reach as
+        far."""
+        p = self._tensor(obj, name, device, kind)
+        if info and hasattr(obj, "get_device"):
+            r = info[0]
             low = high = 0
-            for extent, stride in zip(info[1:1 + r].tolist(), info[1 + r:1 + 2 * r].tolist()):
+            for k in range(1, r + 1):
+                extent, stride = info[k], info[k + r]
                 if extent < 1:
                     return p
                 if stride < 0:
                     low += (extent - 1) * stride
                 else:
                     high += (extent - 1) * stride
+            if low == 0 and high < obj.numel() and obj.is_contiguous():
+                return p
             first = obj.storage_offset()
             if first + low < 0 or (first + high + 1) * obj.element_size() > obj.untyped_storage().nbytes():
                 raise Nd4jError(1, "%s: its shapeInfo reaches beyond the tensor's memory" % name)
@@ -406,12 +437,14 @@ class NativeOps:
     @staticmethod
     def _tads(info, dimension):
         """Number of TADs of an array along a dimension list, and the length of one."""
-        r = int(info[0])
-        axes = {int(ax) % r if r and -r <= ax < r else -1 for ax in dimension}
+        r = info[0]
+        if r == 2 and len(dimension) == 1 and dimension[0] == 1:
+            return info[1], info[2]
+        axes = {ax % r if r and -r <= ax < r else -1 for ax in dimension}
         if -1 in axes:
             raise Nd4jError(1, "dimension %s is not a list of axes of an array of rank %d" % (list(dimension), r))
         count = length = 1
-        for ax, extent in enumerate(info[1:1 + r].tolist()):
+        for ax, extent in enumerate(info[1:1 + r]):
             if ax in axes:
                 length *= extent
             else:
@@ -422,105 +455,128 @@ class NativeOps:
                       dimensionLength):
         """z = (x - mean) * invStd * gain + bias for every TAD of x along `dimension` (nd4jb200_exec_layer_norm). gain,
         bias, mean and invStd may be None."""
-        kind, wide = _KINDS.get(dt), _WIDE.get(dt)
-        xs, xsp = _longs(xShapeInfo)
-        zs, zsp = _longs(zShapeInfo)
-        dm, dmp = _ints(dimension)
-        count, length = self._tads(xs, dm[:dimensionLength])
+        kind, wide, _ = self._kinds(dt)
+        xsp, xl = _descriptor(xShapeInfo)
+        zsp, zl = _descriptor(zShapeInfo)
+        dims = list(dimension)[:dimensionLength]
+        count, length = self._tads(xl, dims)
+        device = self.lib.nd4jb200_get_device()
         self._check(self.lib.nd4jb200_exec_layer_norm(
-            self._stream(extraPointers), dt, self._array(x, "x", kind, xs), xsp, self._tensor(gain, "gain", kind, length),
-            self._tensor(bias, "bias", kind, length), epsilon, self._array(z, "z", kind, zs), zsp,
-            self._tensor(mean, "mean", wide, count), self._tensor(invStd, "invStd", wide, count), dmp, dimensionLength))
+            self._stream(extraPointers), dt, self._array(x, "x", device, kind, xl), xsp,
+            self._tensor(gain, "gain", device, kind, length), self._tensor(bias, "bias", device, kind, length), epsilon,
+            self._array(z, "z", device, kind, zl), zsp, self._tensor(mean, "mean", device, wide, count),
+            self._tensor(invStd, "invStd", device, wide, count), array("i", dims).tobytes(), dimensionLength))
 
     def execLayerNormGrad(self, dt, extraPointers, x, xShapeInfo, gain, mean, invStd, dz, dzShapeInfo, dx, dxShapeInfo, dGain,
                           dBias, dimension, dimensionLength):
         """Gradients of execLayerNorm (nd4jb200_exec_layer_norm_grad). gain, dx, dGain and dBias may be None."""
-        kind, wide = _KINDS.get(dt), _WIDE.get(dt)
-        xs, xsp = _longs(xShapeInfo)
-        ds, dsp = _longs(dzShapeInfo)
-        os_, osp = _longs(dxShapeInfo)
-        dm, dmp = _ints(dimension)
-        count, length = self._tads(xs, dm[:dimensionLength])
+        kind, wide, _ = self._kinds(dt)
+        xsp, xl = _descriptor(xShapeInfo)
+        dsp, dl = _descriptor(dzShapeInfo)
+        osp, ol = _descriptor(dxShapeInfo)
+        dims = list(dimension)[:dimensionLength]
+        count, length = self._tads(xl, dims)
+        device = self.lib.nd4jb200_get_device()
         self._check(self.lib.nd4jb200_exec_layer_norm_grad(
-            self._stream(extraPointers), dt, self._array(x, "x", kind, xs), xsp, self._tensor(gain, "gain", kind, length),
-            self._tensor(mean, "mean", wide, count), self._tensor(invStd, "invStd", wide, count),
-            self._array(dz, "dz", kind, ds), dsp, self._array(dx, "dx", kind, os_), osp,
-            self._tensor(dGain, "dGain", kind, length), self._tensor(dBias, "dBias", kind, length), dmp, dimensionLength))
+            self._stream(extraPointers), dt, self._array(x, "x", device, kind, xl), xsp,
+            self._tensor(gain, "gain", device, kind, length), self._tensor(mean, "mean", device, wide, count),
+            self._tensor(invStd, "invStd", device, wide, count), self._array(dz, "dz", device, kind, dl), dsp,
+            self._array(dx, "dx", device, kind, ol), osp, self._tensor(dGain, "dGain", device, kind, length),
+            self._tensor(dBias, "dBias", device, kind, length), array("i", dims).tobytes(), dimensionLength))
 
     def execTokenLogProbs(self, dt, extraPointers, logits, logitsShapeInfo, tokens, scale, logProbs, entropy, rowMax, logSum,
                           k=0, topTokens=None, topLogProbs=None):
         """Log probabilities of `tokens` (int64 on the device, one per row) under the rows of the logits, their
         entropies, row statistics and k best entries (nd4jb200_exec_token_log_probs). Results may be None."""
-        kind, wide = _KINDS.get(dt), _WIDE.get(dt)
-        xs, xsp = _longs(logitsShapeInfo)
-        rows = int(xs[1])
+        kind, wide, whole = self._kinds(dt)
+        xsp, xl = _descriptor(logitsShapeInfo)
+        rows = xl[1]
+        device = self.lib.nd4jb200_get_device()
         self._check(self.lib.nd4jb200_exec_token_log_probs(
-            self._stream(extraPointers), dt, self._array(logits, "logits", kind, xs), xsp,
-            self._tensor(tokens, "tokens", "torch.int64", rows), scale, self._tensor(logProbs, "logProbs", wide, rows),
-            self._tensor(entropy, "entropy", wide, rows), self._tensor(rowMax, "rowMax", wide, rows),
-            self._tensor(logSum, "logSum", wide, rows), k, self._tensor(topTokens, "topTokens", "torch.int64", rows * k),
-            self._tensor(topLogProbs, "topLogProbs", wide, rows * k)))
+            self._stream(extraPointers), dt, self._array(logits, "logits", device, kind, xl), xsp,
+            self._tensor(tokens, "tokens", device, whole, rows), scale, self._tensor(logProbs, "logProbs", device, wide, rows),
+            self._tensor(entropy, "entropy", device, wide, rows), self._tensor(rowMax, "rowMax", device, wide, rows),
+            self._tensor(logSum, "logSum", device, wide, rows), k, self._tensor(topTokens, "topTokens", device, whole, rows * k),
+            self._tensor(topLogProbs, "topLogProbs", device, wide, rows * k)))
 
     def execTokenLogProbsGrad(self, dt, extraPointers, logits, logitsShapeInfo, tokens, scale, rowMax, logSum, entropy,
                               gLogProbs, gEntropy, dLogits, dLogitsShapeInfo):
         """Gradient of execTokenLogProbs' log probabilities and entropies (nd4jb200_exec_token_log_probs_grad);
         gLogProbs or gEntropy may be None."""
-        kind, wide = _KINDS.get(dt), _WIDE.get(dt)
-        xs, xsp = _longs(logitsShapeInfo)
-        os_, osp = _longs(dLogitsShapeInfo)
-        rows = int(xs[1])
+        kind, wide, whole = self._kinds(dt)
+        xsp, xl = _descriptor(logitsShapeInfo)
+        osp, ol = _descriptor(dLogitsShapeInfo)
+        rows = xl[1]
+        device = self.lib.nd4jb200_get_device()
         self._check(self.lib.nd4jb200_exec_token_log_probs_grad(
-            self._stream(extraPointers), dt, self._array(logits, "logits", kind, xs), xsp,
-            self._tensor(tokens, "tokens", "torch.int64", rows), scale, self._tensor(rowMax, "rowMax", wide, rows),
-            self._tensor(logSum, "logSum", wide, rows), self._tensor(entropy, "entropy", wide, rows),
-            self._tensor(gLogProbs, "gLogProbs", wide, rows), self._tensor(gEntropy, "gEntropy", wide, rows),
-            self._array(dLogits, "dLogits", kind, os_), osp))
+            self._stream(extraPointers), dt, self._array(logits, "logits", device, kind, xl), xsp,
+            self._tensor(tokens, "tokens", device, whole, rows), scale, self._tensor(rowMax, "rowMax", device, wide, rows),
+            self._tensor(logSum, "logSum", device, wide, rows), self._tensor(entropy, "entropy", device, wide, rows),
+            self._tensor(gLogProbs, "gLogProbs", device, wide, rows), self._tensor(gEntropy, "gEntropy", device, wide, rows),
+            self._array(dLogits, "dLogits", device, kind, ol), osp))
 
     def execEmbedding(self, dt, extraPointers, table, tableShapeInfo, tokens, scale, z, zShapeInfo):
         """Row i of z = scale * row tokens[i] of the table (nd4jb200_exec_embedding)."""
-        kind = _KINDS.get(dt)
-        ts, tsp = _longs(tableShapeInfo)
-        zs, zsp = _longs(zShapeInfo)
+        kind, _, whole = self._kinds(dt)
+        tsp, tl = _descriptor(tableShapeInfo)
+        zsp, zl = _descriptor(zShapeInfo)
+        device = self.lib.nd4jb200_get_device()
         self._check(self.lib.nd4jb200_exec_embedding(
-            self._stream(extraPointers), dt, self._array(table, "table", kind, ts), tsp,
-            self._tensor(tokens, "tokens", "torch.int64", int(zs[1])), scale, self._array(z, "z", kind, zs), zsp))
+            self._stream(extraPointers), dt, self._array(table, "table", device, kind, tl), tsp,
+            self._tensor(tokens, "tokens", device, whole, zl[1]), scale, self._array(z, "z", device, kind, zl), zsp))
 
     def execEmbeddingGrad(self, dt, extraPointers, tokens, scale, dz, dzShapeInfo, grad, gradShapeInfo, accumulate=False):
         """Gradient of the table of execEmbedding (nd4jb200_exec_embedding_grad)."""
-        kind = _KINDS.get(dt)
-        ds, dsp = _longs(dzShapeInfo)
-        gs, gsp = _longs(gradShapeInfo)
+        kind, _, whole = self._kinds(dt)
+        dsp, dl = _descriptor(dzShapeInfo)
+        gsp, gl = _descriptor(gradShapeInfo)
+        device = self.lib.nd4jb200_get_device()
         self._check(self.lib.nd4jb200_exec_embedding_grad(
-            self._stream(extraPointers), dt, self._tensor(tokens, "tokens", "torch.int64", int(ds[1])), scale,
-            self._array(dz, "dz", kind, ds), dsp, self._array(grad, "grad", kind, gs), gsp, 1 if accumulate else 0))
+            self._stream(extraPointers), dt, self._tensor(tokens, "tokens", device, whole, dl[1]), scale,
+            self._array(dz, "dz", device, kind, dl), dsp, self._array(grad, "grad", device, kind, gl), gsp,
+            1 if accumulate else 0))
 
-    def _tensorList(self, arrays, name, kind, lengths, n):
+    def _tensorList(self, arrays, name, device, kind, lengths):
+        """Host array of the addresses of device arrays; torch tensors are checked as in _tensor."""
+        n = len(lengths)
         if len(arrays) < n:
-            raise Nd4jError(1, "%s holds fewer than %d tensors" % (name, n))
-        def address(p):
-            return p.value if isinstance(p, ctypes.c_void_p) else p
-        return (ctypes.c_void_p * n)(*[address(self._tensor(t, name, kind, m)) for t, m in zip(arrays[:n], lengths)])
+            raise Nd4jError(1, "%s: fewer than %d tensors" % (name, n))
+        arrays = arrays[:n]
+        if n and device >= 0 and "torch" in sys.modules:
+            T = sys.modules["torch"].Tensor
+            try:
+                # the usual case, one pass per property instead of one per tensor
+                if (list(map(T.numel, arrays)) == lengths and all(map(T.is_contiguous, arrays)) and
+                        set(map(T.get_device, arrays)) == {device} and {t.dtype for t in arrays} == {kind}):
+                    return array("Q", map(T.data_ptr, arrays)).tobytes()
+            except TypeError:
+                pass                                    # not all of them are tensors
+        addresses = [self._tensor(t, name, device, kind, m) for t, m in zip(arrays, lengths)]
+        return array("Q", [(p.value if isinstance(p, ctypes.c_void_p) else p) or 0 for p in addresses]).tobytes()
 
     def execGlobalNorm(self, dt, extraPointers, x, lengths, n, norm):
         """norm = the Euclidean norm over all values of the n tensors in the list x (nd4jb200_exec_global_norm)."""
-        ls, lsp = _longs(lengths)
-        if len(ls) < n:
+        kind, wide, _ = self._kinds(dt)
+        lsp, counts = _descriptor(lengths)
+        if len(counts) < n:
             raise Nd4jError(1, "fewer lengths than tensors")
+        device = self.lib.nd4jb200_get_device()
         self._check(self.lib.nd4jb200_exec_global_norm(self._stream(extraPointers), dt,
-                                                       self._tensorList(x, "a tensor of x", _KINDS.get(dt), ls.tolist(), n), lsp, n,
-                                                       self._tensor(norm, "norm", _WIDE.get(dt), 1)))
+                                                       self._tensorList(x, "a tensor of x", device, kind, counts[:n]), lsp, n,
+                                                       self._tensor(norm, "norm", device, wide, 1)))
 
     def execClipByGlobalNorm(self, dt, extraPointers, x, z, lengths, n, maxNorm, norm):
         """z[i] = x[i] * min(1, maxNorm / norm) over the lists x and z of n tensors, z None for in place
         (nd4jb200_exec_clip_by_global_norm); norm receives the global norm of x."""
-        ls, lsp = _longs(lengths)
-        if len(ls) < n:
+        kind, wide, _ = self._kinds(dt)
+        lsp, counts = _descriptor(lengths)
+        if len(counts) < n:
             raise Nd4jError(1, "fewer lengths than tensors")
-        counts = ls.tolist()
-        zs = None if z is None else self._tensorList(z, "a tensor of z", _KINDS.get(dt), counts, n)
+        device = self.lib.nd4jb200_get_device()
+        zs = None if z is None else self._tensorList(z, "a tensor of z", device, kind, counts[:n])
         self._check(self.lib.nd4jb200_exec_clip_by_global_norm(self._stream(extraPointers), dt,
-                                                               self._tensorList(x, "a tensor of x", _KINDS.get(dt), counts, n), zs,
-                                                               lsp, n, maxNorm, self._tensor(norm, "norm", _WIDE.get(dt), 1)))
+                                                               self._tensorList(x, "a tensor of x", device, kind, counts[:n]), zs,
+                                                               lsp, n, maxNorm, self._tensor(norm, "norm", device, wide, 1)))
 
     def _execMetaPredicateShape(self, dt, extras, opTypeA, opNumA, opTypeB, opNumB, N, dx, xShapeInfo, dy, yShapeInfo,
                                 dz, zShapeInfo, extraA, extraB, scalarA, scalarB):
