@@ -21,7 +21,7 @@
 //
 // Best alternatives need no second sweep: each thread already knows the largest value of its slice and, with a batch
 // number kept beside it, where it stands. The k-th best of these is a lower bound for the k-th best of all; only the
-// slices of the k threads at or above it are read again (k / 512 of the row, mostly from L2), what reaches the bound is
+// slices of the k threads at or above it are read again (k / 256 of the row, mostly from L2), what reaches the bound is
 // collected and ranked by counting. Equal values are ordered by index. Should the collection overflow, or the row hold a
 // NaN (which ranks first), the best are taken one by one.
 #include "../../include/nd4j_b200.h"
@@ -35,8 +35,12 @@ namespace cg = cooperative_groups;
 namespace nd4jb200 {
 namespace {
 
-constexpr int kLpThreads = 512;
-constexpr int kLpWarps = kLpThreads / 32;
+// Threads per CTA. 256 with six CTAs per SM keep their loads overlapping one another's sums (4096 rows of 32768 floats:
+// 94 us; 512 threads, three CTAs: 94; two, the next batch fetched ahead: 107; 8192 rows of 50001 halves: 152, 182, 205).
+// A warp of its own takes a row of up to 512 words (8192 rows of 1000 floats: 37 us with 256 threads).
+constexpr int kLpThreads = 256;
+constexpr int kLpShortWords = 512;
+template <class T> constexpr int lp_ctas(int threads) { return threads == 32 ? 24 : (sizeof(T) == 8 ? 4 : 6); }
 constexpr int kLpBatch = 4;                 // 128-bit words a thread has in flight
 constexpr int kLpMaxTop = 64;
 constexpr int kLpList = 1024;               // collected candidates, at most
@@ -72,6 +76,9 @@ template <> struct LpMath<double> {
     static ND_D double gap(double a, double b, double c) { return (a - b) * c; }
     static ND_D double off(double, double, double) { return 0.0; }
 };
+// the larger of two, a number before a NaN
+ND_D float lp_max(float a, float b) { return fmaxf(a, b); }
+ND_D double lp_max(double a, double b) { return fmax(a, b); }
 ND_D float lp_exp(float d) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d)); return r; }
 ND_D double lp_exp(double d) { return exp(d); }
 ND_D float lp_log(float s) { return log2f(s); }
@@ -121,170 +128,241 @@ template <class T, int V> struct LpRow {
         if constexpr (V == 1) v[0] = x[(LL) word * col];
         else *reinterpret_cast<uint4 *>(v) = __ldcs(reinterpret_cast<const uint4 *>(x + index(word)));
     }
-    // Element f of the slice of thread `slot` in a row shared by `span` threads: (index, value) handed to `f`, ascending.
-    template <class F> ND_D void each(int slot, int span, int firstWord, int wordStep, F f) const {
-        if (V > 1 && firstWord == 0 && slot < head) f(slot, Elem<T>::to_c(at(slot)));
-        for (int w = slot + firstWord * span; w < words; w += wordStep * span) {
+    // The elements of the slice of thread `slot` in a row shared by `span` threads: (index, value) handed to `f`, ascending.
+    template <class F> ND_D void each(int slot, int span, F f) const {
+        if (V > 1 && slot < head) f(slot, Elem<T>::to_c(at(slot)));
+        for (int w = slot; w < words; w += span) {
             alignas(16) T v[V];
             load(w, v);
 #pragma unroll
             for (int k = 0; k < V; k++) f(index(w) + k, Elem<T>::to_c(v[k]));
         }
-        if (V > 1 && firstWord == 0 && slot < tail) f(index(words) + slot, Elem<T>::to_c(at(index(words) + slot)));
+        if (V > 1 && slot < tail) f(index(words) + slot, Elem<T>::to_c(at(index(words) + slot)));
+    }
+};
+
+// Largest of the words of a batch.
+template <class T, int V, int N> ND_D typename LpMath<T>::C lp_batch_max(const T (&v)[N][V]) {
+    typedef typename LpMath<T>::C C;
+    if constexpr (sizeof(T) == 2 && V > 1) {
+        const __half2 *h = reinterpret_cast<const __half2 *>(&v[0][0]);
+        __half2 m = h[0];
+#pragma unroll
+        for (int j = 1; j < N * V / 2; j++) m = __hmax2(m, h[j]);
+        const float lo = __low2float(m), hi = __high2float(m);
+        return lp_max(lp_max(lo, hi), -C(INFINITY));                // all NaN: nothing
+    } else {
+        C m = -C(INFINITY);
+#pragma unroll
+        for (int j = 0; j < N; j++)
+#pragma unroll
+            for (int k = 0; k < V; k++) m = lp_max(m, Elem<T>::to_c(v[j][k]));
+        return m;
+    }
+}
+
+// Moves sums from one reference point to another. A reference far below leaves a power of 0: its sum must not meet an
+// infinite gap.
+template <class T, bool ENT> ND_D void lp_move(typename LpMath<T>::C &s, typename LpMath<T>::C &u, typename LpMath<T>::C from,
+                                               typename LpMath<T>::C to, typename LpMath<T>::C c) {
+    typedef typename LpMath<T>::C C;
+    const C g = LpMath<T>::gap(from, to, c), f = lp_exp(g);
+    if (ENT) u = f == C(0) ? C(0) : f * fma(lp_finite(g), s, u);
+    s *= f;
+}
+
+// A candidate as a key that orders like (value, lower index first): the value's bits made order-preserving, a NaN above
+// all, -0 as +0; then the complement of the index. Comparing keys takes two instructions, which the ranking by counting
+// below lives on. The least key stands for "none": -inf never becomes a candidate.
+template <class C> struct LpKey;
+template <> struct LpKey<float> {
+    unsigned long long k;
+    static ND_D LpKey none() { return LpKey{0ull}; }
+    static ND_D LpKey of(float v, int i) {
+        const unsigned b = __float_as_uint(v + 0.f);
+        const unsigned o = v != v ? 0xffffffffu : b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
+        return LpKey{((unsigned long long) o << 32) | (0xffffffffu - (unsigned) i)};
+    }
+    ND_D int index() const { return (int) (0xffffffffu - (unsigned) k); }
+    ND_D float value() const {
+        const unsigned o = (unsigned) (k >> 32);
+        return o == 0xffffffffu ? __uint_as_float(0x7fffffffu) : __uint_as_float(o ^ ((o >> 31) ? 0x80000000u : 0xffffffffu));
+    }
+    ND_D bool above(const LpKey &o) const { return k > o.k; }
+    ND_D bool same(const LpKey &o) const { return k == o.k; }
+    // the greatest of the warp
+    ND_D LpKey warp_best() const {
+        const unsigned hi = __reduce_max_sync(0xffffffffu, (unsigned) (k >> 32));
+        const unsigned lo = __reduce_max_sync(0xffffffffu, (unsigned) (k >> 32) == hi ? (unsigned) k : 0u);
+        return LpKey{((unsigned long long) hi << 32) | lo};
+    }
+};
+template <> struct LpKey<double> {
+    unsigned long long k;
+    unsigned i;                                   // complement of the index
+    static ND_D LpKey none() { return LpKey{0ull, 0u}; }
+    static ND_D LpKey of(double v, int i) {
+        const unsigned long long b = (unsigned long long) __double_as_longlong(v + 0.0);
+        const unsigned long long o = v != v ? ~0ull : b ^ ((b >> 63) ? ~0ull : 0x8000000000000000ull);
+        return LpKey{o, 0xffffffffu - (unsigned) i};
+    }
+    ND_D int index() const { return (int) (0xffffffffu - i); }
+    ND_D double value() const {
+        return __longlong_as_double(k == ~0ull ? 0x7fffffffffffffffll : (long long) (k ^ ((k >> 63) ? 0x8000000000000000ull : ~0ull)));
+    }
+    ND_D bool above(const LpKey &o) const { return k > o.k || (k == o.k && i > o.i); }
+    ND_D bool same(const LpKey &o) const { return k == o.k && i == o.i; }
+    ND_D LpKey warp_best() const {
+        LpKey b = *this;
+        for (int m = 16; m > 0; m >>= 1) {
+            const LpKey o = {__shfl_xor_sync(0xffffffffu, b.k, m), __shfl_xor_sync(0xffffffffu, b.i, m)};
+            if (o.above(b)) b = o;
+        }
+        return b;
     }
 };
 
 template <class C> struct LpSum { C ref, s, u; };
 
-template <class T, bool ENT> ND_D LpSum<typename LpMath<T>::C> lp_join(const LpSum<typename LpMath<T>::C> &a,
-                                                                       const LpSum<typename LpMath<T>::C> &b, typename LpMath<T>::C c) {
-    typedef LpMath<T> M;
-    typedef typename M::C C;
-    LpSum<C> r;
-    r.ref = a.ref > b.ref ? a.ref : b.ref;
-    const C ga = M::gap(a.ref, r.ref, c), gb = M::gap(b.ref, r.ref, c);
-    const C fa = lp_exp(ga), fb = lp_exp(gb);
-    r.s = a.s * fa + b.s * fb;
-    r.u = C(0);
-    // a reference far below leaves a power of 0: its sum must not meet an infinite gap
-    if (ENT) r.u = (fa == C(0) ? C(0) : fa * (a.u + lp_finite(ga) * a.s)) + (fb == C(0) ? C(0) : fb * (b.u + lp_finite(gb) * b.s));
-    return r;
-}
-
-// Order of candidates: larger first, then the lower index; a NaN before all values.
-template <class C> ND_D bool lp_better(C v, int i, C w, int j) {
-    const bool nv = v != v, nw = w != w;
-    if (nv || nw) return nv && nw ? i < j : nv;
-    return v > w || (v == w && i < j);
-}
-template <class C> ND_D void lp_warp_best(C &v, int &i) {
-    for (int m = 16; m > 0; m >>= 1) {
-        const C w = __shfl_xor_sync(0xffffffffu, v, m);
-        const int j = __shfl_xor_sync(0xffffffffu, i, m);
-        if (j != kLpNone && (i == kLpNone || lp_better(w, j, v, i))) { v = w; i = j; }
-    }
-}
-
-template <class C> struct LpShared {
-    LpSum<C> sums[kLpWarps];
-    LpSum<C> ctaSum;                         // read by the other CTAs of a cluster
-    C warpV[kLpWarps]; int warpI[kLpWarps];
-    C listV[kLpList]; int listI[kLpList];    // candidates
-    C bestV[kLpMaxTop]; int bestI[kLpMaxTop];   // this CTA's best, in order (read by the leading CTA of a cluster)
+template <class C, int LT> struct LpShared {
+    static constexpr int kLpWarps = LT / 32;
+    C sums[kLpWarps], sumsU[kLpWarps], tops[kLpWarps];
+    C ctaMax, ctaS, ctaU;                    // read by the other CTAs of a cluster
+    LpKey<C> warpBest[kLpWarps];
+    LpKey<C> list[kLpList];                  // candidates
+    LpKey<C> best[kLpMaxTop];                // this CTA's best, in order (read by the leading CTA of a cluster)
     int slots[kLpMaxTop];
-    int count, best, numSlots;
+    int counts[8];
+    int count, numBest;
 };
 
-// The k best of the CTA's part of a row into s.bestV / bestI, their number into s.best. (v, i): the thread's own best
-// (i = kLpNone: nothing above -inf). `odd`: the row holds a NaN or +inf.
-template <class T, int V>
-ND_D void lp_select(const LpRow<T, V> &row, typename LpMath<T>::C v, int i, bool odd, int k, int rank, int span, LpShared<typename LpMath<T>::C> &s) {
+// How many of the n keys of a list in shared memory are above `mine`.
+template <class C> ND_D int lp_rank(const LpKey<C> *list, int n, const LpKey<C> &mine) {
+    int above = 0, q = 0;
+    for (; q + 8 <= n; q += 8) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) above += list[q + e].above(mine);
+    }
+    for (; q < n; q++) above += list[q].above(mine);
+    return above;
+}
+
+// The k best of the CTA's part of a row into s.best, their number into s.numBest. `mine`: the thread's own best (none:
+// nothing above -inf). `odd`: the row holds a NaN or +inf.
+template <class T, int V, int LT>
+ND_D void lp_select(const LpRow<T, V> &row, const LpKey<typename LpMath<T>::C> &mine, bool odd, int k, int rank, int span,
+                    LpShared<typename LpMath<T>::C, LT> &s) {
+    constexpr int kLpWarps = LT / 32;
     typedef typename LpMath<T>::C C;
+    typedef LpKey<C> Key;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int slot = rank * kLpThreads + threadIdx.x;
-    if (threadIdx.x == 0) s.count = s.best = s.numSlots = 0;
-    __syncthreads();
+    const int slot = rank * LT + threadIdx.x;
+    const Key none = Key::none();
     bool slow = odd;
     if (!odd) {
         // a first bound: of every warp the r-th best, of these the least; at least r * kLpWarps >= k threads reach it
         const int rounds = (k + kLpWarps - 1) / kLpWarps;
-        C bv = v; int bi = i;
-        bool out = false;
+        Key left = mine, bound = none;
         for (int q = 0; q < rounds; q++) {
-            bv = v; bi = out ? kLpNone : i;
-            lp_warp_best(bv, bi);
-            if (bi == i) out = true;
+            bound = left.warp_best();
+            if (bound.same(left)) left = none;
         }
-        if (lane == 0) { s.warpV[warp] = bv; s.warpI[warp] = bi; }
+        if (lane == 0) s.warpBest[warp] = bound;
+        if (threadIdx.x == 0) s.count = 0;
         __syncthreads();
-        bool all = false;                      // some warp has fewer: every thread with a value counts
-        bv = s.warpV[0]; bi = s.warpI[0];
-        for (int w = 0; w < kLpWarps; w++) {
-            if (s.warpI[w] == kLpNone) all = true;
-            else if (lp_better(bv, bi, s.warpV[w], s.warpI[w])) { bv = s.warpV[w]; bi = s.warpI[w]; }
-        }
-        const bool source = i != kLpNone && (all || !lp_better(bv, bi, v, i));
-        int at = 0;
-        if (source) { at = atomicAdd(&s.count, 1); s.listV[at] = v; s.listI[at] = i; }
+#pragma unroll
+        for (int w = 0; w < kLpWarps; w++) if (bound.above(s.warpBest[w])) bound = s.warpBest[w];
+        // (a warp with fewer values gives none: then every thread with a value counts)
+        const bool source = mine.above(none) && !bound.above(mine);
+        if (source) s.list[atomicAdd(&s.count, 1)] = mine;
         __syncthreads();
         // the k-th best of them exactly
         const int n0 = s.count;
-        int place = 0;
-        if (source) {
-            for (int q = 0; q < n0; q++) if (lp_better(s.listV[q], s.listI[q], v, i)) place++;
-            if (place < k) s.slots[place] = threadIdx.x;
-            if (place == k - 1) { s.warpV[0] = v; s.warpI[0] = i; }
-        }
+        const int place = source ? lp_rank(s.list, n0, mine) : k;
         __syncthreads();
-        const int numSlots = n0 < k ? n0 : k;
-        const bool bounded = n0 >= k;
-        const C tv = s.warpV[0]; const int ti = s.warpI[0];
+        if (place < k) s.slots[place] = threadIdx.x;
+        if (place == k - 1) s.warpBest[0] = mine;
         if (threadIdx.x == 0) s.count = 0;
         __syncthreads();
-        // what reaches it, from the slices of those threads; a slice is read by a warp
-        for (int q = warp; q < numSlots; q += kLpWarps) {
-            const int owner = rank * kLpThreads + s.slots[q];
-            row.each(owner, span, lane, 32, [&](int j, C w) {
-                if (w > -C(INFINITY) && (!bounded || !lp_better(tv, ti, w, j))) {
-                    const int p = atomicAdd(&s.count, 1);
-                    if (p < kLpList) { s.listV[p] = w; s.listI[p] = j; }
-                }
-            });
+        const int numSlots = n0 < k ? n0 : k;
+        const Key least = n0 < k ? none : s.warpBest[0];
+        // what reaches it, from the slices of those threads; every word of them is a thread's
+        auto offer = [&](int j, C w) {
+            const Key key = Key::of(w, j);
+            if (w > -C(INFINITY) && !least.above(key)) {
+                const int p = atomicAdd(&s.count, 1);
+                if (p < kLpList) s.list[p] = key;
+            }
+        };
+        const int perSlot = (row.words + span - 1) / span + 1;          // the first: elements beside the words
+        for (int item = threadIdx.x; item < numSlots * perSlot; item += LT) {
+            const int q = item / perSlot, e = item - q * perSlot;
+            const int owner = rank * LT + s.slots[q];
+            if (e == 0) {
+                if (V > 1 && owner < row.head) offer(owner, Elem<T>::to_c(row.at(owner)));
+                if (V > 1 && owner < row.tail) offer(row.index(row.words) + owner, Elem<T>::to_c(row.at(row.index(row.words) + owner)));
+            } else if (owner + (e - 1) * span < row.words) {
+                const int w = owner + (e - 1) * span;
+                alignas(16) T x[V];
+                row.load(w, x);
+#pragma unroll
+                for (int f = 0; f < V; f++) offer(row.index(w) + f, Elem<T>::to_c(x[f]));
+            }
         }
         __syncthreads();
         const int n = s.count;
         slow = n > kLpList;
         if (!slow) {
-            for (int q = threadIdx.x; q < n; q += kLpThreads) {
-                const C w = s.listV[q]; const int j = s.listI[q];
-                int before = 0;
-                for (int o = 0; o < n && before < k; o++) if (lp_better(s.listV[o], s.listI[o], w, j)) before++;
-                if (before < k) { s.bestV[before] = w; s.bestI[before] = j; }
+            for (int q = threadIdx.x; q < n; q += LT) {
+                const Key key = s.list[q];
+                const int at = lp_rank(s.list, n, key);
+                if (at < k) s.best[at] = key;
             }
-            if (threadIdx.x == 0) s.best = n < k ? n : k;
+            if (threadIdx.x == 0) s.numBest = n < k ? n : k;
         }
         __syncthreads();
     }
     if (!slow) return;
     // one by one: the best of the threads' bests is taken, its owner looks for its next
-    C popV = C(0); int popI = kLpNone;
-    C bv = C(0); int bi = kLpNone;
+    Key pop = none, next = none;
+    bool first = true;
     auto look = [&]() {
-        bi = kLpNone;
-        row.each(slot, span, 0, 1, [&](int j, C w) {
-            const bool real = w > -C(INFINITY) || w != w;
-            if (real && (popI == kLpNone || lp_better(popV, popI, w, j)) && (bi == kLpNone || lp_better(w, j, bv, bi))) { bv = w; bi = j; }
+        next = none;
+        row.each(slot, span, [&](int j, C w) {
+            if (!(w > -C(INFINITY)) && w == w) return;
+            const Key key = Key::of(w, j);
+            if ((first || pop.above(key)) && key.above(next)) next = key;
         });
     };
     look();
+    first = false;
     int taken = 0;
     for (; taken < k; taken++) {
-        C wv = bv; int wi = bi;
-        lp_warp_best(wv, wi);
-        if (lane == 0) { s.warpV[warp] = wv; s.warpI[warp] = wi; }
+        Key b = next.warp_best();
+        if (lane == 0) s.warpBest[warp] = b;
         __syncthreads();
-        wv = s.warpV[0]; wi = s.warpI[0];
-        for (int w = 1; w < kLpWarps; w++)
-            if (s.warpI[w] != kLpNone && (wi == kLpNone || lp_better(s.warpV[w], s.warpI[w], wv, wi))) { wv = s.warpV[w]; wi = s.warpI[w]; }
+#pragma unroll
+        for (int w = 0; w < kLpWarps; w++) if (s.warpBest[w].above(b)) b = s.warpBest[w];
         __syncthreads();
-        if (wi == kLpNone) break;
-        if (threadIdx.x == 0) { s.bestV[taken] = wv; s.bestI[taken] = wi; }
-        popV = wv; popI = wi;
-        if (bi == wi) look();
+        if (!b.above(none)) break;
+        if (threadIdx.x == 0) s.best[taken] = b;
+        pop = b;
+        if (next.same(b)) look();
     }
-    if (threadIdx.x == 0) s.best = taken;
+    if (threadIdx.x == 0) s.numBest = taken;
     __syncthreads();
 }
 
-template <class T, int V, bool ENT, bool TOP>
-__global__ void __launch_bounds__(kLpThreads) k_token_log_probs(const LpArgs a) {
+template <class T, int V, bool ENT, bool TOP, int LT>
+__global__ void __launch_bounds__(LT, lp_ctas<T>(LT)) k_token_log_probs(const LpArgs a) {
     grid_dependency_sync();
     typedef LpMath<T> M;
     typedef typename M::C C;
-    __shared__ LpShared<C> s;
+    constexpr int kLpWarps = LT / 32;
+    __shared__ LpShared<C, LT> s;
     cg::cluster_group cl = cg::this_cluster();
     const int ctas = a.cluster, rank = ctas > 1 ? (int) cl.block_rank() : 0;
-    const int span = ctas * kLpThreads, slot = rank * kLpThreads + threadIdx.x;
+    const int span = ctas * LT, slot = rank * LT + threadIdx.x;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const C c = (C) (a.scale * M::kUnit), back = (C) (1.0 / M::kUnit);
     const C nan = (C) NAN;
@@ -298,9 +376,9 @@ __global__ void __launch_bounds__(kLpThreads) k_token_log_probs(const LpArgs a) 
                     if (a.rowMax) static_cast<C *>(a.rowMax)[r] = C(0);
                     if (a.logSum) static_cast<C *>(a.logSum)[r] = C(0);
                 }
-                if (TOP && threadIdx.x < a.k) {
-                    a.topTokens[r * a.k + threadIdx.x] = -1;
-                    static_cast<C *>(a.topLogProbs)[r * a.k + threadIdx.x] = C(0);
+                for (int q = threadIdx.x; TOP && q < a.k; q += LT) {
+                    a.topTokens[r * a.k + q] = -1;
+                    static_cast<C *>(a.topLogProbs)[r * a.k + q] = C(0);
                 }
             }
             continue;
@@ -308,24 +386,21 @@ __global__ void __launch_bounds__(kLpThreads) k_token_log_probs(const LpArgs a) 
         const LpRow<T, V> row(a, r);
         C top = -C(INFINITY);
         int batch = kLpNone;                                    // where `top` was met: a word, or -1 head, -2 tail
-        LpSum<C> sum = {M::ref(top, c), C(0), C(0)};
+        C ref = M::ref(top, c), sum = C(0), sumU = C(0);
         auto meet = [&](C bm, int where) {
             if (bm > top) {
-                const C ref = M::ref(bm, c);
-                const LpSum<C> moved = {ref, C(0), C(0)};
-                if (ref > sum.ref) sum = lp_join<T, ENT>(sum, moved, c);
+                const C to = M::ref(bm, c);
+                if (to > ref) { lp_move<T, ENT>(sum, sumU, ref, to, c); ref = to; }
                 top = bm;
                 batch = where;
             }
         };
-        auto add = [&](C x) {
-            const C d = M::dist(x, sum.ref, c), e = lp_exp(d);
-            sum.s += e;
-            if (ENT) sum.u = fma(e, lp_finite(d), sum.u);
+        auto add = [&](C x, C &s0, C &u0) {
+            const C d = M::dist(x, ref, c), e = lp_exp(d);
+            s0 += e;
+            if (ENT) u0 = fma(e, lp_finite(d), u0);
         };
-        if (V > 1 && slot < row.head) { const C x = Elem<T>::to_c(row.at(slot)); meet(x, -1); add(x); }
-        for (int w = slot; w < row.words; w += kLpBatch * span) {
-            alignas(16) T v[kLpBatch][V];
+        auto fetch = [&](int w, T (&v)[kLpBatch][V]) {
             if (w + (kLpBatch - 1) * span < row.words) {
 #pragma unroll
                 for (int j = 0; j < kLpBatch; j++) row.load(w + j * span, v[j]);
@@ -339,47 +414,67 @@ __global__ void __launch_bounds__(kLpThreads) k_token_log_probs(const LpArgs a) 
                     }
                 }
             }
-            C bm = -C(INFINITY);
+        };
+        if (V > 1 && slot < row.head) { const C x = Elem<T>::to_c(row.at(slot)); meet(x, -1); add(x, sum, sumU); }
+        alignas(16) T v[kLpBatch][V];
+        for (int w = slot; w < row.words; w += kLpBatch * span) {
+            fetch(w, v);
+            meet(lp_batch_max<T, V, kLpBatch>(v), w);
+            C s1 = C(0), u1 = C(0);                             // two chains of additions
 #pragma unroll
-            for (int j = 0; j < kLpBatch; j++)
+            for (int j = 0; j < kLpBatch; j += 2)
 #pragma unroll
-                for (int k = 0; k < V; k++) { const C x = Elem<T>::to_c(v[j][k]); bm = x > bm ? x : bm; }
-            meet(bm, w);
-#pragma unroll
-            for (int j = 0; j < kLpBatch; j++)
-#pragma unroll
-                for (int k = 0; k < V; k++) add(Elem<T>::to_c(v[j][k]));
+                for (int k = 0; k < V; k++) {
+                    add(Elem<T>::to_c(v[j][k]), sum, sumU);
+                    add(Elem<T>::to_c(v[j + 1][k]), s1, u1);
+                }
+            sum += s1;
+            if (ENT) sumU += u1;
         }
-        if (V > 1 && slot < row.tail) { const C x = Elem<T>::to_c(row.at(row.index(row.words) + slot)); meet(x, -2); add(x); }
+        if (V > 1 && slot < row.tail) { const C x = Elem<T>::to_c(row.at(row.index(row.words) + slot)); meet(x, -2); add(x, sum, sumU); }
 
-        // over the warp, the CTA, the cluster: every thread ends with the row's sums and maximum
-        LpSum<C> all = sum;
+        // over the warp, the CTA, the cluster: first the maximum, then the sums relative to it; every thread gets both
         C m = top;
-        for (int o = 16; o > 0; o >>= 1) {
-            LpSum<C> b;
-            b.ref = __shfl_xor_sync(0xffffffffu, all.ref, o);
-            b.s = __shfl_xor_sync(0xffffffffu, all.s, o);
-            if (ENT) b.u = __shfl_xor_sync(0xffffffffu, all.u, o);
-            // the lower lane's state on the left, so that both sides round alike
-            all = (lane & o) == 0 ? lp_join<T, ENT>(all, b, c) : lp_join<T, ENT>(b, all, c);
-            const C mo = __shfl_xor_sync(0xffffffffu, m, o);
-            m = mo > m ? mo : m;
-        }
+        for (int o = 16; o > 0; o >>= 1) m = lp_max(m, __shfl_xor_sync(0xffffffffu, m, o));
         __syncthreads();                                        // the shared block may still serve the row before
-        if (lane == 0) { s.sums[warp] = all; s.warpV[warp] = m; }
+        if (lane == 0) s.tops[warp] = m;
         __syncthreads();
-        all = s.sums[0];
-        m = s.warpV[0];
-        for (int w = 1; w < kLpWarps; w++) { all = lp_join<T, ENT>(all, s.sums[w], c); m = s.warpV[w] > m ? s.warpV[w] : m; }
+#pragma unroll
+        for (int w = 0; w < kLpWarps; w++) m = lp_max(m, s.tops[w]);
+        LpSum<C> all = {M::ref(m, c), sum, sumU};
+        lp_move<T, ENT>(all.s, all.u, ref, all.ref, c);
+        for (int o = 16; o > 0; o >>= 1) {
+            all.s += __shfl_xor_sync(0xffffffffu, all.s, o);
+            if (ENT) all.u += __shfl_xor_sync(0xffffffffu, all.u, o);
+        }
+        if (lane == 0) { s.sums[warp] = all.s; s.sumsU[warp] = all.u; }
+        __syncthreads();
+        all.s = all.u = C(0);
+#pragma unroll
+        for (int w = 0; w < kLpWarps; w++) { all.s += s.sums[w]; if (ENT) all.u += s.sumsU[w]; }
         if (ctas > 1) {
-            if (threadIdx.x == 0) { s.ctaSum = all; s.bestV[0] = m; }
+            if (threadIdx.x == 0) { s.ctaMax = m; s.ctaS = all.s; s.ctaU = all.u; }
             cl.sync();
-            for (int q = 0; q < ctas; q++) {
-                const LpShared<C> *o = cl.map_shared_rank(&s, q);
-                const LpSum<C> b = o->ctaSum;
-                const C mo = o->bestV[0];
-                all = q == 0 ? b : lp_join<T, ENT>(all, b, c);
-                m = mo > m ? mo : m;
+            // eight independent reads of the other CTAs' shared memory, then the arithmetic
+            C qm[8], qs[8], qu[8];
+#pragma unroll
+            for (int q = 0; q < 8; q++) {
+                const LpShared<C, LT> *o = cl.map_shared_rank(&s, q < ctas ? q : 0);
+                qm[q] = o->ctaMax;
+                qs[q] = o->ctaS;
+                qu[q] = ENT ? o->ctaU : C(0);
+            }
+#pragma unroll
+            for (int q = 0; q < 8; q++) m = lp_max(m, qm[q]);
+            all.ref = M::ref(m, c);
+            all.s = all.u = C(0);
+#pragma unroll
+            for (int q = 0; q < 8; q++) {
+                if (q < ctas) {
+                    lp_move<T, ENT>(qs[q], qu[q], M::ref(qm[q], c), all.ref, c);
+                    all.s += qs[q];
+                    all.u += qu[q];
+                }
             }
             cl.sync();
         }
@@ -405,50 +500,40 @@ __global__ void __launch_bounds__(kLpThreads) k_token_log_probs(const LpArgs a) 
             if (batch == -1) mine = slot;
             else if (batch == -2) mine = row.index(row.words) + slot;
             else if (batch != kLpNone) {
-                for (int j = kLpBatch - 1; j >= 0; j--) {
-                    if (batch + j * span < row.words) {
-                        alignas(16) T v[V];
-                        row.load(batch + j * span, v);
+                fetch(batch, v);
 #pragma unroll
-                        for (int k = V - 1; k >= 0; k--) if (Elem<T>::to_c(v[k]) == top) mine = row.index(batch + j * span) + k;
-                    }
-                }
+                for (int j = kLpBatch - 1; j >= 0; j--)
+#pragma unroll
+                    for (int k = V - 1; k >= 0; k--) if (Elem<T>::to_c(v[j][k]) == top) mine = row.index(batch + j * span) + k;
             }
-            lp_select<T, V>(row, top, mine, odd, a.k, rank, span, s);
+            typedef LpKey<C> Key;
+            lp_select<T, V, LT>(row, mine == kLpNone ? Key::none() : Key::of(top, mine), odd, a.k, rank, span, s);
             if (ctas > 1) {
                 cl.sync();
                 if (rank == 0) {
                     // the CTAs' lists, at most 8 * 64 entries, ranked once more
-                    __shared__ int counts[8];
-                    if (threadIdx.x < ctas) counts[threadIdx.x] = cl.map_shared_rank(&s, threadIdx.x)->best;
+                    if (threadIdx.x < ctas) s.counts[threadIdx.x] = cl.map_shared_rank(&s, threadIdx.x)->numBest;
                     __syncthreads();
-                    const int q = threadIdx.x / kLpMaxTop, e = threadIdx.x - q * kLpMaxTop;
-                    int first = 0, n = 0;
-                    for (int o = 0; o < ctas; o++) { if (o < q) first += counts[o]; n += counts[o]; }
-                    const bool have = q < ctas && e < counts[q];
-                    if (have) {
-                        const LpShared<C> *o = cl.map_shared_rank(&s, q);
-                        s.listV[first + e] = o->bestV[e];
-                        s.listI[first + e] = o->bestI[e];
+                    int n = 0;
+                    for (int q = 0; q < ctas; q++) {
+                        for (int e = threadIdx.x; e < s.counts[q]; e += LT) s.list[n + e] = cl.map_shared_rank(&s, q)->best[e];
+                        n += s.counts[q];
                     }
                     __syncthreads();
-                    int before = 0;
-                    C w = C(0); int j = 0;
-                    if (have) {
-                        w = s.listV[first + e]; j = s.listI[first + e];
-                        for (int o = 0; o < n; o++) if (lp_better(s.listV[o], s.listI[o], w, j)) before++;
+                    for (int e = threadIdx.x; e < n; e += LT) {
+                        const Key key = s.list[e];
+                        const int at = lp_rank(s.list, n, key);
+                        if (at < a.k) s.best[at] = key;
                     }
-                    __syncthreads();
-                    if (have && before < a.k) { s.bestV[before] = w; s.bestI[before] = j; }
-                    if (threadIdx.x == 0) s.best = n < a.k ? n : a.k;
+                    if (threadIdx.x == 0) s.numBest = n < a.k ? n : a.k;
                     __syncthreads();
                 }
             }
             if (rank == 0) {
-                const int n = s.best;
-                for (int q = threadIdx.x; q < n; q += kLpThreads) {
-                    a.topTokens[r * a.k + q] = s.bestI[q];
-                    static_cast<C *>(a.topLogProbs)[r * a.k + q] = odd ? nan : log_p(s.bestV[q]);
+                const int n = s.numBest;
+                for (int q = threadIdx.x; q < n; q += LT) {
+                    a.topTokens[r * a.k + q] = s.best[q].index();
+                    static_cast<C *>(a.topLogProbs)[r * a.k + q] = odd ? nan : log_p(s.best[q].value());
                 }
                 // fewer values than asked for: masked entries follow, the first of them first
                 if (n < a.k && warp == 0) {
@@ -541,9 +626,9 @@ __global__ void __launch_bounds__(kLpGradThreads) k_token_log_probs_grad(const L
 }
 
 // ---- host side ---------------------------------------------------------------------------------------------------
-template <class K> void launch_log_probs(K kernel, const LpArgs &a, unsigned grid, cudaStream_t st) {
+template <class K> void launch_log_probs(K kernel, const LpArgs &a, unsigned grid, int threads, cudaStream_t st) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid); cfg.blockDim = dim3(kLpThreads); cfg.stream = st;
+    cfg.gridDim = dim3(grid); cfg.blockDim = dim3((unsigned) threads); cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -555,26 +640,32 @@ template <class K> void launch_log_probs(K kernel, const LpArgs &a, unsigned gri
     count_launch();
 }
 
-template <class T, int V> void lp_forward_kernels(const LpArgs &a, unsigned grid, cudaStream_t st) {
+template <class T, int V, int LT> void lp_forward_kernels(const LpArgs &a, unsigned grid, cudaStream_t st) {
     if (a.k > 0) {
-        if (a.entropy) launch_log_probs(k_token_log_probs<T, V, true, true>, a, grid, st);
-        else launch_log_probs(k_token_log_probs<T, V, false, true>, a, grid, st);
+        if (a.entropy) launch_log_probs(k_token_log_probs<T, V, true, true, LT>, a, grid, LT, st);
+        else launch_log_probs(k_token_log_probs<T, V, false, true, LT>, a, grid, LT, st);
     } else {
-        if (a.entropy) launch_log_probs(k_token_log_probs<T, V, true, false>, a, grid, st);
-        else launch_log_probs(k_token_log_probs<T, V, false, false>, a, grid, st);
+        if (a.entropy) launch_log_probs(k_token_log_probs<T, V, true, false, LT>, a, grid, LT, st);
+        else launch_log_probs(k_token_log_probs<T, V, false, false, LT>, a, grid, LT, st);
     }
 }
 
 template <class T> Status lp_forward(LpArgs &a, cudaStream_t st) {
     constexpr int V = Elem<T>::kVec;
-    // Rows that would leave SMs idle are shared by a cluster, as long as every CTA keeps at least two batches.
+    // Rows that would leave SMs idle are shared by a cluster, as long as every CTA keeps at least one batch.
     a.cluster = 1;
-    const LL perCta = (LL) kLpThreads * kLpBatch * (a.col == 1 ? V : 1) * 2;
-    while (a.cluster < 8 && a.rows * a.cluster * 2 <= kNumSMs * 2 && a.vocab >= a.cluster * 2 * perCta) a.cluster *= 2;
+    const LL run = a.col == 1 ? V : 1;
+    const LL perCta = (LL) kLpThreads * kLpBatch * run;
+    const bool shortRows = a.col == 1 && a.vocab <= kLpShortWords * run;
+    while (!shortRows && a.cluster < 8 && a.rows * a.cluster * 2 <= kNumSMs * 2 && a.vocab >= a.cluster * 2 * perCta) a.cluster *= 2;
     LL grid = a.rows * a.cluster;
     if (grid > 0x7fffffff / 8 * 8) grid = 0x7fffffff / 8 * 8;
-    if (a.col == 1) lp_forward_kernels<T, V>(a, (unsigned) grid, st);
-    else lp_forward_kernels<T, 1>(a, (unsigned) grid, st);
+    if (a.col == 1) {
+        if (shortRows) lp_forward_kernels<T, V, 32>(a, (unsigned) grid, st);
+        else lp_forward_kernels<T, V, kLpThreads>(a, (unsigned) grid, st);
+    } else {
+        lp_forward_kernels<T, 1, kLpThreads>(a, (unsigned) grid, st);
+    }
     ND_CUDA(cudaGetLastError());
     return kOk;
 }
