@@ -127,14 +127,31 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) k_ln_forward(const LnArgs a
 template <class C> struct LnPair { C a, b; };
 
 // Backward over rows held by groups of G threads (several groups per CTA when rows are short). Each thread holds the
-// same columns of every row it meets, and therefore their sums of dg and db. The next row is read while the sums of
-// this one travel: a group waits once per row, on a barrier of its own.
-template <class T, int V, int NP>
-__global__ void __launch_bounds__(512) k_ln_backward(const LnArgs a, const int G) {
+// same columns of every row it meets, and therefore their sums of dg and db; a group waits once per row, on a barrier of
+// its own. Rows are fetched D iterations ahead by asynchronous copies into shared memory, which holds far more of them
+// in flight than registers could (65536 rows of 1024 floats: 163 us with one row ahead in registers).
+//
+// OWN: every thread copies the very words that it will read, so that nothing but its own copies has to be waited for;
+// needs words of 4, 8 or 16 bytes. Otherwise (half rows of odd length or offset) the group copies the aligned 16-byte
+// words that a row lies in and every thread picks its columns from them behind a barrier.
+template <int BYTES> ND_D void ln_copy(void *to, const void *from) {
+    const unsigned s = (unsigned) __cvta_generic_to_shared(to);
+    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(s), "l"(from) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(s), "l"(from), "n"(BYTES) : "memory");
+}
+ND_D void ln_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> ND_D void ln_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+ND_D void ln_group_barrier(int group, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(threads) : "memory"); }
+
+// Bytes that one staged row may take: its words, one more for the shift, kept to whole words.
+inline ND_HD int ln_staged(LL cols, int elem) { return (int) ((cols * elem + 15) / 16 * 16 + 16); }
+
+template <class T, int V, int NP, int D, int MAXT, int CTAS, bool OWN>
+__global__ void __launch_bounds__(MAXT, CTAS) k_ln_backward(const LnArgs a, const int G) {
     grid_dependency_sync();
     typedef typename Elem<T>::C C;
     extern __shared__ __align__(16) unsigned char ln_smem[];
-    __shared__ LnPair<C> slots[2][16];
+    __shared__ LnPair<C> slots[2][MAXT / 32];
     const int groups = blockDim.x / G, group = threadIdx.x / G, t = threadIdx.x - group * G;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, firstWarp = group * (G >> 5), warps = G >> 5;
     const int words = (int) (a.cols / V);
@@ -155,27 +172,71 @@ __global__ void __launch_bounds__(512) k_ln_backward(const LnArgs a, const int G
         }
     }
     const LL step = (LL) gridDim.x * groups;
-    LL r = (LL) blockIdx.x * groups + group;
-    LnWord<T, V> wx[NP], wd[NP];
-    C mean = C(0), inv = C(0);
-    auto read = [&](LL row) {
-        const T *x = px + row * a.xRow, *d = pdz + row * a.dzRow;
+    const int staged = OWN ? 0 : ln_staged(a.cols, sizeof(T));
+
+    // where stage d keeps word j of array q for this thread, or (not OWN) array q of this group
+    auto own = [&](int d, int q, int j) { return reinterpret_cast<LnWord<T, V> *>(ln_smem) + ((d * 2 + q) * NP + j) * blockDim.x + threadIdx.x; };
+    auto shared = [&](int d, int q) { return ln_smem + ((d * 2 + q) * groups + group) * staged; };
+    auto shift = [](const T *row) { return (int) (reinterpret_cast<unsigned long long>(row) & 15); };
+    auto fetch = [&](int d, LL row) {
+        if (row < a.rows) {
+            const T *src[2] = {px + row * a.xRow, pdz + row * a.dzRow};
 #pragma unroll
-        for (int j = 0; j < NP; j++)
-            if (t + G * j < words) { wx[j].load(x + (t + G * j) * V); wd[j].load(d + (t + G * j) * V); }
-        mean = pMean[row]; inv = pInv[row];
+            for (int q = 0; q < 2; q++) {
+                if constexpr (OWN) {
+#pragma unroll
+                    for (int j = 0; j < NP; j++)
+                        if (t + G * j < words) ln_copy<sizeof(T) * V>(own(d, q, j), src[q] + (t + G * j) * V);
+                } else {
+                    const int off = shift(src[q]), bytes = (int) a.cols * (int) sizeof(T);
+                    const char *from = reinterpret_cast<const char *>(src[q]) - off;
+                    unsigned char *to = shared(d, q);
+                    // the words wholly inside the row are copied as such, the at most two others element by element
+                    for (int w = t; w * 16 < off + bytes; w += G) {
+                        if (w * 16 >= off && w * 16 + 16 <= off + bytes) ln_copy<16>(to + w * 16, from + w * 16);
+                        else {
+#pragma unroll
+                            for (int e = 0; e < 16; e += (int) sizeof(T)) {
+                                const int at = w * 16 + e;
+                                if (at >= off && at < off + bytes) *reinterpret_cast<T *>(to + at) = *reinterpret_cast<const T *>(from + at);
+                            }
+                        }
+                    }
+                }
+            }
+        }
+        ln_commit();
     };
-    if (r < a.rows) read(r);
+    LL r = (LL) blockIdx.x * groups + group;
+    C mean = C(0), inv = C(0);
+    if (r < a.rows) { mean = pMean[r]; inv = pInv[r]; }
+#pragma unroll
+    for (int d = 0; d < D; d++) fetch(d, r + d * step);
+    int stage = 0;
     for (int parity = 0; r < a.rows; r += step, parity ^= 1) {
+        C nextMean = C(0), nextInv = C(0);
+        if (r + step < a.rows) { nextMean = pMean[r + step]; nextInv = pInv[r + step]; }
+        ln_wait<D - 1>();
+        const T *sx = nullptr, *sd = nullptr;
+        if constexpr (!OWN) {
+            ln_group_barrier(group, G);                        // everyone's copies of this row stand
+            sx = reinterpret_cast<const T *>(shared(stage, 0) + shift(px + r * a.xRow));
+            sd = reinterpret_cast<const T *>(shared(stage, 1) + shift(pdz + r * a.dzRow));
+        }
         C h[NP][V], d[NP][V];
         LnPair<C> s = {C(0), C(0)};
 #pragma unroll
         for (int j = 0; j < NP; j++) {
             const bool in = t + G * j < words;
+            LnWord<T, V> wx, wd;
+            if (in) {
+                if constexpr (OWN) { wx = *own(stage, 0, j); wd = *own(stage, 1, j); }
+                else { wx.v[0] = sx[t + G * j]; wd.v[0] = sd[t + G * j]; }
+            }
 #pragma unroll
             for (int k = 0; k < V; k++) {
-                h[j][k] = in ? (Elem<T>::to_c(wx[j].v[k]) - mean) * inv : C(0);
-                const C dz = in ? Elem<T>::to_c(wd[j].v[k]) : C(0);
+                h[j][k] = in ? (Elem<T>::to_c(wx.v[k]) - mean) * inv : C(0);
+                const C dz = in ? Elem<T>::to_c(wd.v[k]) : C(0);
                 sg[j][k] = fma(dz, h[j][k], sg[j][k]);
                 sb[j][k] += dz;
                 d[j][k] = dz * gain[j][k];
@@ -183,17 +244,17 @@ __global__ void __launch_bounds__(512) k_ln_backward(const LnArgs a, const int G
                 s.b = fma(d[j][k], h[j][k], s.b);
             }
         }
-        const C thisInv = inv;
-        if (r + step < a.rows) read(r + step);
+        if (OWN) fetch(stage, r + D * step);                   // these words have been read
+        s.a = ln_warp_sum(s.a);
+        s.b = ln_warp_sum(s.b);
+        if (warps > 1 || !OWN) {
+            if (lane == 0) slots[parity][warp] = s;
+            ln_group_barrier(group, G);
+            s = slots[parity][firstWarp];
+            for (int k = 1; k < warps; k++) { s.a += slots[parity][firstWarp + k].a; s.b += slots[parity][firstWarp + k].b; }
+        }
+        if (!OWN) fetch(stage, r + D * step);                  // nobody reads this stage any more
         if (pdx) {
-            s.a = ln_warp_sum(s.a);
-            s.b = ln_warp_sum(s.b);
-            if (warps > 1) {
-                if (lane == 0) slots[parity][warp] = s;
-                asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(G) : "memory");
-                s = slots[parity][firstWarp];
-                for (int k = 1; k < warps; k++) { s.a += slots[parity][firstWarp + k].a; s.b += slots[parity][firstWarp + k].b; }
-            }
             s.a *= invN; s.b *= invN;
             T *dx = pdx + r * a.zRow;
 #pragma unroll
@@ -201,16 +262,20 @@ __global__ void __launch_bounds__(512) k_ln_backward(const LnArgs a, const int G
                 if (t + G * j < words) {
                     LnWord<T, V> o;
 #pragma unroll
-                    for (int k = 0; k < V; k++) o.v[k] = Elem<T>::from_c(thisInv * (d[j][k] - s.a - h[j][k] * s.b));
+                    for (int k = 0; k < V; k++) o.v[k] = Elem<T>::from_c(inv * (d[j][k] - s.a - h[j][k] * s.b));
                     o.store(dx + (t + G * j) * V);
                 }
             }
         }
+        mean = nextMean; inv = nextInv;
+        stage = stage + 1 == D ? 0 : stage + 1;
     }
+    ln_wait<0>();
     if (!a.dGain && !a.dBias) return;
     // the CTA's groups add up in shared memory, one after the other, then the CTA's sums become a partial row
     C *pg = static_cast<C *>(a.partials) + (LL) blockIdx.x * 2 * a.cols, *pb = pg + a.cols;
     C *tg = reinterpret_cast<C *>(ln_smem), *tb = tg + a.cols;
+    __syncthreads();                                           // the stages have been read by all groups
     for (int q = 0; q < groups; q++) {
         if (q == group) {
 #pragma unroll
@@ -242,7 +307,15 @@ __global__ void __launch_bounds__(1024) k_ln_fold(const LnArgs a) {
     const C *p = static_cast<const C *>(a.partials);
     C g = C(0), b = C(0);
     if (c < a.cols) {
-        for (int q = warp; q < a.numPartials; q += 32) { g += p[(LL) q * 2 * a.cols + c]; b += p[((LL) q * 2 + 1) * a.cols + c]; }
+        int q = warp;
+        for (; q + 96 < a.numPartials; q += 128) {              // eight loads in flight
+            C vg[4], vb[4];
+#pragma unroll
+            for (int u = 0; u < 4; u++) { vg[u] = p[(LL) (q + 32 * u) * 2 * a.cols + c]; vb[u] = p[((LL) (q + 32 * u) * 2 + 1) * a.cols + c]; }
+#pragma unroll
+            for (int u = 0; u < 4; u++) { g += vg[u]; b += vb[u]; }
+        }
+        for (; q < a.numPartials; q += 32) { g += p[(LL) q * 2 * a.cols + c]; b += p[((LL) q * 2 + 1) * a.cols + c]; }
     }
     tg[warp][lane] = g; tb[warp][lane] = b;
     __syncthreads();
@@ -398,12 +471,17 @@ template <class K> inline void launch_with_smem(K kernel, dim3 grid, dim3 block,
     count_launch();
 }
 
-template <class T, int V, int NP> Status ln_backward_rows(LnArgs &a, int G, cudaStream_t st) {
+// Launches the kernel for rows of unit stride: `block` threads in groups of G, D stages of rows in shared memory.
+template <class T, int V, int NP, int D, int MAXT, int CTAS, bool OWN>
+Status ln_backward_rows(LnArgs &a, int G, int block, cudaStream_t st) {
     typedef typename Elem<T>::C C;
-    const int block = G < 256 ? 256 / G * G : G;
     const int groups = block / G;
-    const size_t smem = groups > 1 ? 2 * (size_t) a.cols * sizeof(C) : 0;
-    LL grid = (LL) kNumSMs * (block <= 256 ? 3 : 1);
+    const size_t stages = OWN ? (size_t) D * 2 * NP * V * sizeof(T) * block : (size_t) D * 2 * groups * ln_staged(a.cols, sizeof(T));
+    const size_t fold = groups > 1 ? 2 * (size_t) a.cols * sizeof(C) : 0;
+    const size_t smem = stages > fold ? stages : fold;
+    auto kernel = k_ln_backward<T, V, NP, D, MAXT, CTAS, OWN>;
+    if (smem > 48 * 1024 - 512) ND_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem));
+    LL grid = (LL) kNumSMs * CTAS;
     if (grid > ceil_div(a.rows, groups)) grid = ceil_div(a.rows, groups);
     a.numPartials = (int) grid;
     Scratch scratch(st);
@@ -412,21 +490,27 @@ template <class T, int V, int NP> Status ln_backward_rows(LnArgs &a, int G, cuda
         ND_TRY(scratch.alloc((size_t) grid * 2 * (size_t) a.cols * sizeof(C)));
         a.partials = scratch.at<void>(0);
     }
-    launch_with_smem(k_ln_backward<T, V, NP>, dim3((unsigned) grid), dim3((unsigned) block), smem, st, a, G);
+    launch_with_smem(kernel, dim3((unsigned) grid), dim3((unsigned) block), smem, st, a, G);
     if (weights) launch_kernel(k_ln_fold<T>, dim3((unsigned) ceil_div(a.cols, 32)), dim3(1024), st, a);
     ND_CUDA(cudaGetLastError());
     return kOk;
 }
 
+// V values per word and per copy. Up to 256 threads of kSmall values a CTA takes several rows at a time and shares the
+// SM with two others; longer rows take a CTA, and twice the values per thread once 512 threads do not hold them.
+template <class T, int V, bool OWN> Status ln_backward_fit(LnArgs &a, cudaStream_t st) {
+    typedef LnFit<T> F;
+    constexpr int kStages = sizeof(T) == 2 ? 6 : 4;          // 192 KB per SM for float and double, 144 KB for half
+    if (int G = threads_for(a.cols, F::kSmall, 256)) return ln_backward_rows<T, V, F::kSmall / V, kStages, 256, 3, OWN>(a, G, 256 / G * G, st);
+    if (int G = threads_for(a.cols, F::kSmall, 512)) return ln_backward_rows<T, V, F::kSmall / V, kStages, 512, 1, OWN>(a, G, G, st);
+    return ln_backward_rows<T, V, F::kMid / V, 3, 512, 1, OWN>(a, threads_for(a.cols, F::kMid, 512), threads_for(a.cols, F::kMid, 512), st);
+}
+
 template <class T> Status ln_backward(LnArgs &a, bool rows, bool words, cudaStream_t st) {
     typedef typename Elem<T>::C C;
-    typedef LnFit<T> F;
-    constexpr int V = Elem<T>::kVec;
-    if (rows && a.rows > 0) {
-        if (int G = threads_for(a.cols, F::kSmall, 512))
-            return words ? ln_backward_rows<T, V, F::kSmall / V>(a, G, st) : ln_backward_rows<T, 1, F::kSmall>(a, G, st);
-        if (int G = threads_for(a.cols, F::kMid, 512))
-            return words ? ln_backward_rows<T, V, F::kMid / V>(a, G, st) : ln_backward_rows<T, 1, F::kMid>(a, G, st);
+    if (rows && a.rows > 0 && threads_for(a.cols, LnFit<T>::kMid, 512)) {
+        if (words) return ln_backward_fit<T, Elem<T>::kVec, true>(a, st);
+        return ln_backward_fit<T, 1, sizeof(T) >= 4>(a, st);
     }
     Scratch scratch(st);
     if (a.dGain || a.dBias) {
