@@ -42,19 +42,20 @@ template <class T, int V> struct LnRun {
     T v[V];
     ND_D void load(const T *p) {
         if constexpr (V == 1) v[0] = *p;
+        else if constexpr (V * sizeof(T) == 4) *reinterpret_cast<unsigned *>(v) = *reinterpret_cast<const unsigned *>(p);
         else *reinterpret_cast<uint4 *>(v) = *reinterpret_cast<const uint4 *>(p);
     }
     ND_D void store(T *p) const {
         if constexpr (V == 1) *p = v[0];
+        else if constexpr (V * sizeof(T) == 4) *reinterpret_cast<unsigned *>(p) = *reinterpret_cast<const unsigned *>(v);
         else *reinterpret_cast<uint4 *>(p) = *reinterpret_cast<const uint4 *>(v);
     }
 };
-template <class T, int V> struct alignas(V == 1 ? sizeof(T) : 16) LnWord : LnRun<T, V> {};
+template <class T, int V> struct alignas(V * sizeof(T)) LnWord : LnRun<T, V> {};
 
-// Sum over the CTA (or the warp, when a row belongs to one warp), the same bits in every thread.
-template <bool WARP, class C> ND_D C ln_row_sum(C v, C *slots) {
+// Sum over the CTA, the same bits in every thread.
+template <class C> ND_D C ln_row_sum(C v, C *slots) {
     v = ln_warp_sum(v);
-    if (WARP) return v;
     const int warps = blockDim.x >> 5;
     __syncthreads();                                  // slots may still be read from the sum before
     if ((threadIdx.x & 31) == 0) slots[threadIdx.x >> 5] = v;
@@ -64,80 +65,77 @@ template <bool WARP, class C> ND_D C ln_row_sum(C v, C *slots) {
     return r;
 }
 
-// A row in the registers of a warp (WARP) or of the whole CTA: NP words of V values per thread, thread t holding words
-// t, t + G, ...
-template <class T, int V, int NP, bool WARP>
-__global__ void __launch_bounds__(WARP ? 256 : 1024) k_ln_forward(const LnArgs a) {
-    grid_dependency_sync();
+// Two floats that one instruction adds or multiplies (add / mul / fma.rn.f32x2: each half rounds like the scalar
+// instruction); a single double. Half rows are bound by the issue of instructions, which this halves.
+template <class C> struct LnPack;
+template <> struct LnPack<float> {
+    static constexpr int W = 2;
+    unsigned long long v;
+    static ND_D LnPack of(float a, float b) { LnPack r; asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b)); return r; }
+    static ND_D LnPack all(float a) { return of(a, a); }
+    ND_D float get(int k) const {
+        float a, b;
+        asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+        return k ? b : a;
+    }
+    ND_D float sum() const { return get(0) + get(1); }
+    static ND_D LnPack add(LnPack a, LnPack b) { LnPack r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v)); return r; }
+    static ND_D LnPack mul(LnPack a, LnPack b) { LnPack r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v)); return r; }
+    static ND_D LnPack fma(LnPack a, LnPack b, LnPack c) { LnPack r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v)); return r; }
+};
+template <> struct LnPack<double> {
+    static constexpr int W = 1;
+    double v;
+    static ND_D LnPack all(double a) { return LnPack{a}; }
+    ND_D double get(int) const { return v; }
+    ND_D double sum() const { return v; }
+    static ND_D LnPack add(LnPack a, LnPack b) { return LnPack{a.v + b.v}; }
+    static ND_D LnPack mul(LnPack a, LnPack b) { return LnPack{a.v * b.v}; }
+    static ND_D LnPack fma(LnPack a, LnPack b, LnPack c) { return LnPack{::fma(a.v, b.v, c.v)}; }
+};
+// The values of a thread's NP words as packs, `beyond` where there is no word, and back.
+template <class T, int V, int NP> struct LnVals {
     typedef typename Elem<T>::C C;
-    __shared__ C slots[32];
-    const int G = WARP ? 32 : blockDim.x;
-    const int t = WARP ? threadIdx.x & 31 : threadIdx.x;
-    const LL first = WARP ? (LL) blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
-    const LL step = WARP ? (LL) gridDim.x * (blockDim.x >> 5) : gridDim.x;
-    const int words = (int) (a.cols / V);
-    const C n = (C) a.cols;
-    const T *gain = static_cast<const T *>(a.gain), *bias = static_cast<const T *>(a.bias);
-    for (LL r = first; r < a.rows; r += step) {
-        const T *x = static_cast<const T *>(a.x) + r * a.xRow;
-        T *z = static_cast<T *>(a.z) + r * a.zRow;
-        LnWord<T, V> w[NP];
-        C sum = C(0);
+    typedef LnPack<C> P;
+    static constexpr int N = NP * V / P::W;
+    static_assert(NP * V % P::W == 0, "a thread holds whole packs");
+    P p[N];
+    ND_D void zero() {
 #pragma unroll
-        for (int j = 0; j < NP; j++) if (t + G * j < words) w[j].load(x + (LL) (t + G * j) * V);
-        C v[NP][V];
+        for (int i = 0; i < N; i++) p[i] = P::all(C(0));
+    }
+    template <class W> ND_D void from(const W (&w)[NP], int live, C beyond = C(0)) {      // `live`: values that exist
 #pragma unroll
-        for (int j = 0; j < NP; j++) {
-            const bool in = t + G * j < words;
+        for (int i = 0; i < N; i++) {
+            C e[P::W];
 #pragma unroll
-            for (int k = 0; k < V; k++) { v[j][k] = in ? Elem<T>::to_c(w[j].v[k]) : C(0); sum += v[j][k]; }
-        }
-        const C mean = ln_row_sum<WARP>(sum, slots) / n;
-        C sq = C(0);
-#pragma unroll
-        for (int j = 0; j < NP; j++) {
-            if (t + G * j < words) {
-#pragma unroll
-                for (int k = 0; k < V; k++) { v[j][k] -= mean; sq = fma(v[j][k], v[j][k], sq); }
+            for (int k = 0; k < P::W; k++) {
+                const int at = i * P::W + k;
+                e[k] = at < live ? Elem<T>::to_c(w[at / V].v[at % V]) : beyond;
             }
-        }
-        const C inv = C(1) / sqrt(ln_row_sum<WARP>(sq, slots) / n + (C) a.epsilon);
-        if (t == 0) {
-            if (a.mean) static_cast<C *>(a.mean)[r] = mean;
-            if (a.invStd) static_cast<C *>(a.invStd)[r] = inv;
-        }
-#pragma unroll
-        for (int j = 0; j < NP; j++) {
-            const int c = (t + G * j) * V;
-            if (t + G * j < words) {
-                LnWord<T, V> g, b, o;
-                if (gain) g.load(gain + c);
-                if (bias) b.load(bias + c);
-#pragma unroll
-                for (int k = 0; k < V; k++) {
-                    const C h = v[j][k] * inv;
-                    o.v[k] = Elem<T>::from_c(fma(h, gain ? Elem<T>::to_c(g.v[k]) : C(1), bias ? Elem<T>::to_c(b.v[k]) : C(0)));
-                }
-                o.store(z + c);
-            }
+            if constexpr (P::W == 2) p[i] = P::of(e[0], e[1]);
+            else p[i] = P::all(e[0]);
         }
     }
-}
+    template <class W> ND_D void to(W (&w)[NP]) const {
+#pragma unroll
+        for (int at = 0; at < NP * V; at++) w[at / V].v[at % V] = Elem<T>::from_c(p[at / P::W].get(at % P::W));
+    }
+};
 
-template <class C> struct LnPair { C a, b; };
-
-// Backward over rows held by groups of G threads (several groups per CTA when rows are short). Each thread holds the
-// same columns of every row it meets, and therefore their sums of dg and db; a group waits once per row, on a barrier of
-// its own. Rows are fetched D iterations ahead by asynchronous copies into shared memory, which holds far more of them
-// in flight than registers could (65536 rows of 1024 floats: 163 us with one row ahead in registers).
+// Rows on their way into shared memory: D iterations ahead by asynchronous copies, which hold far more of them in flight
+// than registers could (backward, 65536 rows of 1024 floats: 163 us with one row ahead in registers, 142 so).
 //
-// OWN: every thread copies the very words that it will read, so that nothing but its own copies has to be waited for;
-// needs words of 4, 8 or 16 bytes. Otherwise (half rows of odd length or offset) the group copies the aligned 16-byte
-// words that a row lies in and every thread picks its columns from them behind a barrier.
-template <int BYTES> ND_D void ln_copy(void *to, const void *from) {
+// kLnOwn: rows of whole, aligned 16-byte words. Every thread copies the very words that it will read, so that nothing but
+// its own copies has to be waited for. Otherwise the group copies the aligned words that a row lies in (and, element by
+// element, what it shares with its neighbours' words), and every thread picks its columns from them behind a barrier;
+// half rows in pairs of columns, which are a 4-byte word in every second row of odd length. kLnFull: as kLnOwn, with every
+// word of every thread inside the row, so that no bounds are kept (forward, 16384 rows of 4096 floats: 28 instructions
+// per value with them).
+enum LnMode { kLnPicked = 0, kLnOwn = 1, kLnFull = 2 };
+ND_D void ln_copy(void *to, const void *from) {
     const unsigned s = (unsigned) __cvta_generic_to_shared(to);
-    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(s), "l"(from) : "memory");
-    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(s), "l"(from), "n"(BYTES) : "memory");
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(s), "l"(from) : "memory");
 }
 ND_D void ln_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> ND_D void ln_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -146,126 +144,246 @@ ND_D void ln_group_barrier(int group, int threads) { asm volatile("bar.sync %0, 
 // Bytes that one staged row may take: its words, one more for the shift, kept to whole words.
 inline ND_HD int ln_staged(LL cols, int elem) { return (int) ((cols * elem + 15) / 16 * 16 + 16); }
 
-template <class T, int V, int NP, int D, int MAXT, int CTAS, bool OWN>
+// A CTA's groups of G threads, each holding one row at a time: thread t the words t, t + G, ... (NP at most) of V values.
+// The row's last word may be cut short: `live` counts the thread's values that exist, the first ones of its words.
+template <class T, int V, int NP, int NA, int MODE> struct LnGroup {
+    static constexpr bool OWN = MODE != kLnPicked, FULL = MODE == kLnFull;
+    unsigned char *smem;
+    int G, groups, group, t, have, live, staged;
+    LL cols;
+    ND_D LnGroup(unsigned char *m, int g, LL c) : smem(m), G(g), cols(c) {
+        groups = blockDim.x / G;
+        group = threadIdx.x / G;
+        t = threadIdx.x - group * G;
+        const int words = (int) ((cols + V - 1) / V);
+        have = t < words ? (words - 1 - t) / G + 1 : 0;
+        live = have * V;
+        if (have > 0 && word(have - 1) == words - 1) live -= words * V - (int) cols;
+        staged = OWN ? 0 : ln_staged(cols, sizeof(T));
+    }
+    ND_D int held() const { return FULL ? NP : have; }
+    ND_D int values() const { return FULL ? NP * V : live; }
+    ND_D int word(int j) const { return t + G * j; }
+    ND_D int column(int at) const { return word(at / V) * V + at % V; }
+    // where stage d keeps word j of array q for this thread, or (not OWN) array q of this group
+    ND_D LnWord<T, V> *own(int d, int q, int j) const {
+        return reinterpret_cast<LnWord<T, V> *>(smem) + ((d * NA + q) * NP + j) * blockDim.x + threadIdx.x;
+    }
+    ND_D unsigned char *shared(int d, int q) const { return smem + ((d * NA + q) * groups + group) * staged; }
+    static ND_D int shift(const T *row) { return (int) (reinterpret_cast<unsigned long long>(row) & 15); }
+    ND_D void fetch(int d, int q, const T *row) const {
+        if constexpr (OWN) {
+#pragma unroll
+            for (int j = 0; j < NP; j++) if (j < held()) ln_copy(own(d, q, j), row + word(j) * V);
+        } else {
+            const int off = shift(row), end = off + (int) cols * (int) sizeof(T), last = end / 16 * 16;
+            const char *from = reinterpret_cast<const char *>(row) - off;
+            unsigned char *to = shared(d, q);
+            for (int w = (off + 15) / 16 * 16 + t * 16; w < last; w += G * 16) ln_copy(to + w, from + w);
+            const int e = t * (int) sizeof(T);                // element of the first and of the last word
+            if (e < 16) {
+                if (e >= off && off > 0 && e < end) *reinterpret_cast<T *>(to + e) = *reinterpret_cast<const T *>(from + e);
+                if (last + e < end && last + e >= off) *reinterpret_cast<T *>(to + last + e) = *reinterpret_cast<const T *>(from + last + e);
+            }
+        }
+    }
+    ND_D void read(int d, int q, const T *row, LnWord<T, V> (&w)[NP]) const {
+        if constexpr (OWN) {
+#pragma unroll
+            for (int j = 0; j < NP; j++) if (j < held()) w[j] = *own(d, q, j);
+        } else {
+            const T *s = reinterpret_cast<const T *>(shared(d, q) + shift(row));
+            pick(s, w);
+        }
+    }
+    // The thread's values of a row at p, which need not be aligned to words (values behind the last are read as well when
+    // `p` is a staged row: its buffer reaches a word further).
+    ND_D void pick(const T *p, LnWord<T, V> (&w)[NP]) const {
+        if (V == 1 || (reinterpret_cast<unsigned long long>(p) & (sizeof(T) * V - 1)) == 0) {
+#pragma unroll
+            for (int j = 0; j < NP; j++) if (j < held()) w[j].load(p + word(j) * V);
+        } else {
+#pragma unroll
+            for (int j = 0; j < NP; j++)
+#pragma unroll
+                for (int k = 0; k < V; k++) if (j < held()) w[j].v[k] = p[word(j) * V + k];
+        }
+    }
+    // The thread's values of a vector in global memory.
+    ND_D void load(const T *p, LnWord<T, V> (&w)[NP]) const {
+#pragma unroll
+        for (int at = 0; at < NP * V; at++) if (at < values()) w[at / V].v[at % V] = p[column(at)];
+    }
+    ND_D void store(T *p, const LnWord<T, V> (&w)[NP]) const {
+        if (OWN || V == 1) {
+#pragma unroll
+            for (int j = 0; j < NP; j++) if (j < held()) w[j].store(p + word(j) * V);
+        } else if ((reinterpret_cast<unsigned long long>(p) & (sizeof(T) * V - 1)) == 0) {
+#pragma unroll
+            for (int j = 0; j < NP; j++) {
+                if (j * V + V <= values()) w[j].store(p + word(j) * V);
+                else if (j * V < values()) p[word(j) * V] = w[j].v[0];
+            }
+        } else {
+#pragma unroll
+            for (int at = 0; at < NP * V; at++) if (at < values()) p[column(at)] = w[at / V].v[at % V];
+        }
+    }
+};
+
+// Sum over the group's warps; `slots` holds one value per warp of the CTA and must not be in use.
+template <int MAXW, class S, class ADD> ND_D S ln_group_sum(S v, S *slots, int group, int G, ADD add) {
+    const int warps = G >> 5, warp = threadIdx.x >> 5;
+    if (warps == 1) return v;
+    if ((threadIdx.x & 31) == 0) slots[warp] = v;
+    ln_group_barrier(group, G);
+    const S *mine = slots + group * warps;
+    S r = mine[0];
+#pragma unroll
+    for (int k = 1; k < MAXW; k++) if (k < warps) r = add(r, mine[k]);
+    return r;
+}
+
+// Forward: two sums per row, the second around the mean. The slots alternate over four sets, so that a set is written
+// again only two barriers after it was read.
+template <class T, int V, int NP, int D, int MAXT, int CTAS, int MODE>
+__global__ void __launch_bounds__(MAXT, CTAS) k_ln_forward(const LnArgs a, const int G) {
+    grid_dependency_sync();
+    typedef typename Elem<T>::C C;
+    typedef LnPack<C> P;
+    typedef LnVals<T, V, NP> Vals;
+    extern __shared__ __align__(16) unsigned char ln_smem[];
+    __shared__ C slots[4][MAXT / 32];
+    constexpr bool OWN = MODE != kLnPicked;
+    const LnGroup<T, V, NP, 1, MODE> g(ln_smem, G, a.cols);
+    const T *px = static_cast<const T *>(a.x);
+    T *pz = static_cast<T *>(a.z);
+    const C invN = C(1) / (C) a.cols;
+    Vals gain, bias;
+    LnWord<T, V> w[NP];
+    if (a.gain) { g.load(static_cast<const T *>(a.gain), w); gain.from(w, g.values()); }
+    if (a.bias) { g.load(static_cast<const T *>(a.bias), w); bias.from(w, g.values()); }
+#pragma unroll
+    for (int i = 0; i < Vals::N; i++) {
+        if (!a.gain) gain.p[i] = P::all(C(1));
+        if (!a.bias) bias.p[i] = P::all(C(0));
+    }
+    const LL step = (LL) gridDim.x * g.groups;
+    LL r = (LL) blockIdx.x * g.groups + g.group;
+#pragma unroll
+    for (int d = 0; d < D; d++) { if (r + d * step < a.rows) g.fetch(d, 0, px + (r + d * step) * a.xRow); ln_commit(); }
+    int stage = 0;
+    auto plus = [](C x, C y) { return x + y; };
+    for (int parity = 0; r < a.rows; r += step, parity ^= 2) {
+        ln_wait<D - 1>();
+        if (!OWN) ln_group_barrier(g.group, G);                // everyone's copies of this row stand
+        g.read(stage, 0, px + r * a.xRow, w);
+        Vals v;
+        v.from(w, g.values());
+        P s = v.p[0];
+#pragma unroll
+        for (int i = 1; i < Vals::N; i++) s = P::add(s, v.p[i]);
+        C sum = ln_group_sum<MAXT / 32>(ln_warp_sum(s.sum()), slots[parity], g.group, G, plus);
+        if (!OWN && (G >> 5) == 1) __syncwarp();
+        // the stage has been read (OWN: by this thread, which alone uses these words; otherwise by all: the barrier)
+        if (r + D * step < a.rows) g.fetch(stage, 0, px + (r + D * step) * a.xRow);
+        ln_commit();
+        const C mean = sum * invN;
+        const P away = P::all(-mean);
+        s = P::all(C(0));
+#pragma unroll
+        for (int i = 0; i < Vals::N; i++) {
+            v.p[i] = P::add(v.p[i], away);
+            const bool whole = i * P::W + P::W <= g.values(), some = i * P::W < g.values();
+            if (whole) s = P::fma(v.p[i], v.p[i], s);
+            else if (some) { if constexpr (P::W == 2) { const P one = P::of(v.p[i].get(0), C(0)); s = P::fma(one, one, s); } }
+        }
+        sum = ln_group_sum<MAXT / 32>(ln_warp_sum(s.sum()), slots[parity + 1], g.group, G, plus);
+        const C inv = C(1) / sqrt(sum * invN + (C) a.epsilon);
+        if (g.t == 0) {
+            if (a.mean) static_cast<C *>(a.mean)[r] = mean;
+            if (a.invStd) static_cast<C *>(a.invStd)[r] = inv;
+        }
+        const P scale = P::all(inv);
+#pragma unroll
+        for (int i = 0; i < Vals::N; i++) v.p[i] = P::fma(P::mul(v.p[i], scale), gain.p[i], bias.p[i]);
+        v.to(w);
+        g.store(pz + r * a.zRow, w);
+        stage = stage + 1 == D ? 0 : stage + 1;
+    }
+    ln_wait<0>();
+}
+
+template <class C> struct LnPair { C a, b; };
+
+// Backward: each thread holds the same columns of every row it meets, and therefore their sums of dg and db; a group
+// waits once per row, on a barrier of its own.
+template <class T, int V, int NP, int D, int MAXT, int CTAS, int MODE>
 __global__ void __launch_bounds__(MAXT, CTAS) k_ln_backward(const LnArgs a, const int G) {
     grid_dependency_sync();
     typedef typename Elem<T>::C C;
+    typedef LnPack<C> P;
+    typedef LnVals<T, V, NP> Vals;
     extern __shared__ __align__(16) unsigned char ln_smem[];
     __shared__ LnPair<C> slots[2][MAXT / 32];
-    const int groups = blockDim.x / G, group = threadIdx.x / G, t = threadIdx.x - group * G;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, firstWarp = group * (G >> 5), warps = G >> 5;
-    const int words = (int) (a.cols / V);
-    const C invN = C(1) / (C) a.cols;
+    constexpr bool OWN = MODE != kLnPicked;
+    const LnGroup<T, V, NP, 2, MODE> g(ln_smem, G, a.cols);
     const T *px = static_cast<const T *>(a.x), *pdz = static_cast<const T *>(a.dz);
     T *pdx = static_cast<T *>(a.z);
     const C *pMean = static_cast<const C *>(a.mean), *pInv = static_cast<const C *>(a.invStd);
-    C gain[NP][V], sg[NP][V], sb[NP][V];
+    const C invN = C(1) / (C) a.cols;
+    Vals gain, sg, sb;
+    LnWord<T, V> w[NP];
+    if (a.gain) { g.load(static_cast<const T *>(a.gain), w); gain.from(w, g.values()); }
+    else {
 #pragma unroll
-    for (int j = 0; j < NP; j++) {
-        LnWord<T, V> g;
-        const bool in = t + G * j < words;
-        if (in && a.gain) g.load(static_cast<const T *>(a.gain) + (t + G * j) * V);
-#pragma unroll
-        for (int k = 0; k < V; k++) {
-            gain[j][k] = in ? (a.gain ? Elem<T>::to_c(g.v[k]) : C(1)) : C(0);
-            sg[j][k] = sb[j][k] = C(0);
-        }
+        for (int i = 0; i < Vals::N; i++) gain.p[i] = P::all(C(1));
     }
-    const LL step = (LL) gridDim.x * groups;
-    const int staged = OWN ? 0 : ln_staged(a.cols, sizeof(T));
-
-    // where stage d keeps word j of array q for this thread, or (not OWN) array q of this group
-    auto own = [&](int d, int q, int j) { return reinterpret_cast<LnWord<T, V> *>(ln_smem) + ((d * 2 + q) * NP + j) * blockDim.x + threadIdx.x; };
-    auto shared = [&](int d, int q) { return ln_smem + ((d * 2 + q) * groups + group) * staged; };
-    auto shift = [](const T *row) { return (int) (reinterpret_cast<unsigned long long>(row) & 15); };
+    sg.zero();
+    sb.zero();
+    const LL step = (LL) gridDim.x * g.groups;
+    LL r = (LL) blockIdx.x * g.groups + g.group;
     auto fetch = [&](int d, LL row) {
-        if (row < a.rows) {
-            const T *src[2] = {px + row * a.xRow, pdz + row * a.dzRow};
-#pragma unroll
-            for (int q = 0; q < 2; q++) {
-                if constexpr (OWN) {
-#pragma unroll
-                    for (int j = 0; j < NP; j++)
-                        if (t + G * j < words) ln_copy<sizeof(T) * V>(own(d, q, j), src[q] + (t + G * j) * V);
-                } else {
-                    const int off = shift(src[q]), bytes = (int) a.cols * (int) sizeof(T);
-                    const char *from = reinterpret_cast<const char *>(src[q]) - off;
-                    unsigned char *to = shared(d, q);
-                    // the words wholly inside the row are copied as such, the at most two others element by element
-                    for (int w = t; w * 16 < off + bytes; w += G) {
-                        if (w * 16 >= off && w * 16 + 16 <= off + bytes) ln_copy<16>(to + w * 16, from + w * 16);
-                        else {
-#pragma unroll
-                            for (int e = 0; e < 16; e += (int) sizeof(T)) {
-                                const int at = w * 16 + e;
-                                if (at >= off && at < off + bytes) *reinterpret_cast<T *>(to + at) = *reinterpret_cast<const T *>(from + at);
-                            }
-                        }
-                    }
-                }
-            }
-        }
+        if (row < a.rows) { g.fetch(d, 0, px + row * a.xRow); g.fetch(d, 1, pdz + row * a.dzRow); }
         ln_commit();
     };
-    LL r = (LL) blockIdx.x * groups + group;
     C mean = C(0), inv = C(0);
     if (r < a.rows) { mean = pMean[r]; inv = pInv[r]; }
 #pragma unroll
     for (int d = 0; d < D; d++) fetch(d, r + d * step);
     int stage = 0;
+    auto plus = [](const LnPair<C> &x, const LnPair<C> &y) { return LnPair<C>{x.a + y.a, x.b + y.b}; };
     for (int parity = 0; r < a.rows; r += step, parity ^= 1) {
         C nextMean = C(0), nextInv = C(0);
         if (r + step < a.rows) { nextMean = pMean[r + step]; nextInv = pInv[r + step]; }
         ln_wait<D - 1>();
-        const T *sx = nullptr, *sd = nullptr;
-        if constexpr (!OWN) {
-            ln_group_barrier(group, G);                        // everyone's copies of this row stand
-            sx = reinterpret_cast<const T *>(shared(stage, 0) + shift(px + r * a.xRow));
-            sd = reinterpret_cast<const T *>(shared(stage, 1) + shift(pdz + r * a.dzRow));
-        }
-        C h[NP][V], d[NP][V];
-        LnPair<C> s = {C(0), C(0)};
+        if (!OWN) ln_group_barrier(g.group, G);                // everyone's copies of this row stand
+        Vals h, d;
+        g.read(stage, 0, px + r * a.xRow, w);
+        h.from(w, g.values(), mean);                               // beyond the row: h = 0, dz = 0
+        g.read(stage, 1, pdz + r * a.dzRow, w);
+        d.from(w, g.values());
+        const P away = P::all(-mean), scale = P::all(inv);
+        P pa = P::all(C(0)), pb = pa;
 #pragma unroll
-        for (int j = 0; j < NP; j++) {
-            const bool in = t + G * j < words;
-            LnWord<T, V> wx, wd;
-            if (in) {
-                if constexpr (OWN) { wx = *own(stage, 0, j); wd = *own(stage, 1, j); }
-                else { wx.v[0] = sx[t + G * j]; wd.v[0] = sd[t + G * j]; }
-            }
-#pragma unroll
-            for (int k = 0; k < V; k++) {
-                h[j][k] = in ? (Elem<T>::to_c(wx.v[k]) - mean) * inv : C(0);
-                const C dz = in ? Elem<T>::to_c(wd.v[k]) : C(0);
-                sg[j][k] = fma(dz, h[j][k], sg[j][k]);
-                sb[j][k] += dz;
-                d[j][k] = dz * gain[j][k];
-                s.a += d[j][k];
-                s.b = fma(d[j][k], h[j][k], s.b);
-            }
+        for (int i = 0; i < Vals::N; i++) {
+            h.p[i] = P::mul(P::add(h.p[i], away), scale);
+            sg.p[i] = P::fma(d.p[i], h.p[i], sg.p[i]);
+            sb.p[i] = P::add(sb.p[i], d.p[i]);
+            d.p[i] = P::mul(d.p[i], gain.p[i]);
+            pa = P::add(pa, d.p[i]);
+            pb = P::fma(d.p[i], h.p[i], pb);
         }
         if (OWN) fetch(stage, r + D * step);                   // these words have been read
-        s.a = ln_warp_sum(s.a);
-        s.b = ln_warp_sum(s.b);
-        if (warps > 1 || !OWN) {
-            if (lane == 0) slots[parity][warp] = s;
-            ln_group_barrier(group, G);
-            s = slots[parity][firstWarp];
-            for (int k = 1; k < warps; k++) { s.a += slots[parity][firstWarp + k].a; s.b += slots[parity][firstWarp + k].b; }
-        }
-        if (!OWN) fetch(stage, r + D * step);                  // nobody reads this stage any more
+        LnPair<C> s = {ln_warp_sum(pa.sum()), ln_warp_sum(pb.sum())};
+        s = ln_group_sum<MAXT / 32>(s, slots[parity], g.group, G, plus);
+        if (!OWN) { if ((G >> 5) == 1) __syncwarp(); fetch(stage, r + D * step); }         // nobody reads this stage any more
         if (pdx) {
-            s.a *= invN; s.b *= invN;
-            T *dx = pdx + r * a.zRow;
+            const P ma = P::all(-s.a * invN), mb = P::all(-s.b * invN);
 #pragma unroll
-            for (int j = 0; j < NP; j++) {
-                if (t + G * j < words) {
-                    LnWord<T, V> o;
-#pragma unroll
-                    for (int k = 0; k < V; k++) o.v[k] = Elem<T>::from_c(inv * (d[j][k] - s.a - h[j][k] * s.b));
-                    o.store(dx + (t + G * j) * V);
-                }
-            }
+            for (int i = 0; i < Vals::N; i++) d.p[i] = P::mul(P::fma(h.p[i], mb, P::add(d.p[i], ma)), scale);
+            d.to(w);
+            g.store(pdx + r * a.zRow, w);
         }
         mean = nextMean; inv = nextInv;
         stage = stage + 1 == D ? 0 : stage + 1;
@@ -276,23 +394,20 @@ __global__ void __launch_bounds__(MAXT, CTAS) k_ln_backward(const LnArgs a, cons
     C *pg = static_cast<C *>(a.partials) + (LL) blockIdx.x * 2 * a.cols, *pb = pg + a.cols;
     C *tg = reinterpret_cast<C *>(ln_smem), *tb = tg + a.cols;
     __syncthreads();                                           // the stages have been read by all groups
-    for (int q = 0; q < groups; q++) {
-        if (q == group) {
+    for (int q = 0; q < g.groups; q++) {
+        if (q == g.group) {
 #pragma unroll
-            for (int j = 0; j < NP; j++) {
-                if (t + G * j < words) {
-#pragma unroll
-                    for (int k = 0; k < V; k++) {
-                        const int c = (t + G * j) * V + k;
-                        C vg = sg[j][k], vb = sb[j][k];
-                        if (q > 0) { vg += tg[c]; vb += tb[c]; }
-                        if (q + 1 < groups) { tg[c] = vg; tb[c] = vb; }
-                        else { pg[c] = vg; pb[c] = vb; }
-                    }
+            for (int at = 0; at < NP * V; at++) {
+                if (at < g.values()) {
+                    const int c = g.column(at);
+                    C vg = sg.p[at / P::W].get(at % P::W), vb = sb.p[at / P::W].get(at % P::W);
+                    if (q > 0) { vg += tg[c]; vb += tb[c]; }
+                    if (q + 1 < g.groups) { tg[c] = vg; tb[c] = vb; }
+                    else { pg[c] = vg; pb[c] = vb; }
                 }
             }
         }
-        if (groups > 1) __syncthreads();
+        if (g.groups > 1) __syncthreads();
     }
 }
 
@@ -344,13 +459,13 @@ __global__ void __launch_bounds__(kLnSweepThreads) k_ln_forward_sweep(const LnAr
         T *z = static_cast<T *>(a.z) + view_offset(a.zOuter, r);
         C s = C(0);
         for (LL c = threadIdx.x; c < a.cols; c += kLnSweepThreads) s += Elem<T>::load(x + view_offset(a.xInner, c));
-        const C mean = ln_row_sum<false>(s, slots) / n;
+        const C mean = ln_row_sum(s, slots) / n;
         s = C(0);
         for (LL c = threadIdx.x; c < a.cols; c += kLnSweepThreads) {
             const C v = Elem<T>::load(x + view_offset(a.xInner, c)) - mean;
             s = fma(v, v, s);
         }
-        const C inv = C(1) / sqrt(ln_row_sum<false>(s, slots) / n + (C) a.epsilon);
+        const C inv = C(1) / sqrt(ln_row_sum(s, slots) / n + (C) a.epsilon);
         if (threadIdx.x == 0) {
             if (a.mean) static_cast<C *>(a.mean)[r] = mean;
             if (a.invStd) static_cast<C *>(a.invStd)[r] = inv;
@@ -382,8 +497,8 @@ __global__ void __launch_bounds__(kLnSweepThreads) k_ln_backward_sweep(const LnA
             sa += d;
             sb = fma(d, h, sb);
         }
-        sa = ln_row_sum<false>(sa, slots) / n;
-        sb = ln_row_sum<false>(sb, slots) / n;
+        sa = ln_row_sum(sa, slots) / n;
+        sb = ln_row_sum(sb, slots) / n;
         for (LL c = threadIdx.x; c < a.cols; c += kLnSweepThreads) {
             const C h = (Elem<T>::load(x + view_offset(a.xInner, c)) - mean) * inv;
             const C d = Elem<T>::load(dz + view_offset(a.dzInner, c)) * (gain ? Elem<T>::load(gain + c) : C(1));
@@ -425,39 +540,26 @@ __global__ void __launch_bounds__(512) k_ln_weights_sweep(const LnArgs a) {
 }
 
 // ---- host side ---------------------------------------------------------------------------------------------------
+// How rows are held: so many values per thread while up to 256 threads hold the row (a CTA then takes as many rows as fit
+// and shares its SM with others), a CTA of up to 512 threads beyond, with twice the values once that is too few. More
+// values per thread spread the work that every row costs a thread; the registers set the limit. Forward: 16 (double: 8).
+// Backward: 8 floats, but 16 halves, whose bytes are fewer for the same instructions (65536 rows of 1024 halves: 124 us
+// with 8 values, 87 with 16), 4 doubles.
 template <class T> struct LnFit {
-    // values per thread the register budget is set for: 32 / 16 of float, half of that of double
-    static constexpr int kBig = sizeof(typename Elem<T>::C) == 8 ? 16 : 32;
-    static constexpr int kMid = kBig / 2;
-    static constexpr int kSmall = kBig / 4;
+    static constexpr int kForward = sizeof(T) == 8 ? 8 : 16;
+    static constexpr int kForwardStages = sizeof(T) == 2 ? 6 : 4;       // 144 .. 192 KB of rows per SM
+    static constexpr int kBackward = sizeof(T) == 8 ? 4 : (sizeof(T) == 4 ? 8 : 16);
+    static constexpr int kBackwardCtas = sizeof(T) == 2 ? 2 : 3;
+    static constexpr int kBackwardStages = sizeof(T) == 2 ? 5 : 4;
+    static constexpr bool kBackwardTwice = sizeof(T) > 2;               // 32 halves and their sums do not fit
+    static constexpr int kBackwardMost = kBackwardTwice ? 2 * kBackward : kBackward;
+    static constexpr int kPick = sizeof(T) == 2 ? 2 : 1;                // values per word of rows that are no whole words
 };
 inline int threads_for(LL cols, int perThread, int most) {
     LL t = ceil_div(ceil_div(cols, perThread), 32) * 32;
     return t > most ? 0 : (int) t;
 }
 inline unsigned grid_for(LL n) { return (unsigned) (n < 0x7fffffffLL ? (n > 0 ? n : 1) : 0x7fffffffLL); }
-
-template <class T, int V> void ln_forward_rows(const LnArgs &a, cudaStream_t st) {
-    typedef LnFit<T> F;
-    // A warp per row needs no barrier; from the length on that 32 threads cannot hold, the CTA shares the row.
-    if (a.cols <= 32 * F::kBig)
-        launch_kernel(k_ln_forward<T, V, F::kBig / V, true>, dim3(grid_for(ceil_div(a.rows, 8))), dim3(256), st, a);
-    else if (int t = threads_for(a.cols, F::kMid, 1024))
-        launch_kernel(k_ln_forward<T, V, F::kMid / V, false>, dim3(grid_for(a.rows)), dim3((unsigned) t), st, a);
-    else
-        launch_kernel(k_ln_forward<T, V, F::kBig / V, false>, dim3(grid_for(a.rows)), dim3(1024), st, a);
-}
-
-template <class T> Status ln_forward(LnArgs &a, bool rows, bool words, cudaStream_t st) {
-    if (rows && a.cols <= 1024 * LnFit<T>::kBig) {
-        if (words) ln_forward_rows<T, Elem<T>::kVec>(a, st);
-        else ln_forward_rows<T, 1>(a, st);
-    } else {
-        launch_kernel(k_ln_forward_sweep<T>, dim3(grid_for(a.rows)), dim3(kLnSweepThreads), st, a);
-    }
-    ND_CUDA(cudaGetLastError());
-    return kOk;
-}
 
 template <class K> inline void launch_with_smem(K kernel, dim3 grid, dim3 block, size_t smem, cudaStream_t st, const LnArgs &a, int G) {
     cudaLaunchConfig_t cfg = {};
@@ -471,15 +573,50 @@ template <class K> inline void launch_with_smem(K kernel, dim3 grid, dim3 block,
     count_launch();
 }
 
+template <class T, int V, int NP, int D, int MAXT, int CTAS, int MODE>
+Status ln_forward_rows(const LnArgs &a, int G, int block, cudaStream_t st) {
+    const int groups = block / G;
+    const size_t smem = MODE != kLnPicked ? (size_t) D * NP * V * sizeof(T) * block : (size_t) D * groups * ln_staged(a.cols, sizeof(T));
+    auto kernel = k_ln_forward<T, V, NP, D, MAXT, CTAS, MODE>;
+    if (smem > 48 * 1024 - 512) ND_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem));
+    LL grid = (LL) kNumSMs * CTAS;
+    if (grid > ceil_div(a.rows, groups)) grid = ceil_div(a.rows, groups);
+    launch_with_smem(kernel, dim3((unsigned) grid), dim3((unsigned) block), smem, st, a, G);
+    ND_CUDA(cudaGetLastError());
+    return kOk;
+}
+
+template <class T, int V, int NP, int D, int MAXT, int CTAS, int MODE>
+Status ln_forward_held(const LnArgs &a, int G, int block, cudaStream_t st) {
+    if (MODE == kLnOwn && a.cols == (LL) G * NP * V) return ln_forward_rows<T, V, NP, D, MAXT, CTAS, MODE == kLnOwn ? kLnFull : MODE>(a, G, block, st);
+    return ln_forward_rows<T, V, NP, D, MAXT, CTAS, MODE>(a, G, block, st);
+}
+
+template <class T, int V, int MODE> Status ln_forward_fit(const LnArgs &a, cudaStream_t st) {
+    constexpr int S = LnFit<T>::kForward, D = LnFit<T>::kForwardStages;
+    if (int G = threads_for(a.cols, S, 256)) return ln_forward_held<T, V, S / V, D, 256, 3, MODE>(a, G, 256 / G * G, st);
+    if (int G = threads_for(a.cols, S, 512)) return ln_forward_held<T, V, S / V, D, 512, 1, MODE>(a, G, G, st);
+    const int G = threads_for(a.cols, 2 * S, 512);
+    return ln_forward_held<T, V, 2 * S / V, 3, 512, 1, MODE>(a, G, G, st);
+}
+
+template <class T> Status ln_forward(LnArgs &a, bool rows, bool words, cudaStream_t st) {
+    if (rows && threads_for(a.cols, 2 * LnFit<T>::kForward, 512))
+        return words ? ln_forward_fit<T, Elem<T>::kVec, kLnOwn>(a, st) : ln_forward_fit<T, LnFit<T>::kPick, kLnPicked>(a, st);
+    launch_kernel(k_ln_forward_sweep<T>, dim3(grid_for(a.rows)), dim3(kLnSweepThreads), st, a);
+    ND_CUDA(cudaGetLastError());
+    return kOk;
+}
+
 // Launches the kernel for rows of unit stride: `block` threads in groups of G, D stages of rows in shared memory.
-template <class T, int V, int NP, int D, int MAXT, int CTAS, bool OWN>
+template <class T, int V, int NP, int D, int MAXT, int CTAS, int MODE>
 Status ln_backward_rows(LnArgs &a, int G, int block, cudaStream_t st) {
     typedef typename Elem<T>::C C;
     const int groups = block / G;
-    const size_t stages = OWN ? (size_t) D * 2 * NP * V * sizeof(T) * block : (size_t) D * 2 * groups * ln_staged(a.cols, sizeof(T));
+    const size_t stages = MODE != kLnPicked ? (size_t) D * 2 * NP * V * sizeof(T) * block : (size_t) D * 2 * groups * ln_staged(a.cols, sizeof(T));
     const size_t fold = groups > 1 ? 2 * (size_t) a.cols * sizeof(C) : 0;
     const size_t smem = stages > fold ? stages : fold;
-    auto kernel = k_ln_backward<T, V, NP, D, MAXT, CTAS, OWN>;
+    auto kernel = k_ln_backward<T, V, NP, D, MAXT, CTAS, MODE>;
     if (smem > 48 * 1024 - 512) ND_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem));
     LL grid = (LL) kNumSMs * CTAS;
     if (grid > ceil_div(a.rows, groups)) grid = ceil_div(a.rows, groups);
@@ -496,22 +633,28 @@ Status ln_backward_rows(LnArgs &a, int G, int block, cudaStream_t st) {
     return kOk;
 }
 
-// V values per word and per copy. Up to 256 threads of kSmall values a CTA takes several rows at a time and shares the
-// SM with two others; longer rows take a CTA, and twice the values per thread once 512 threads do not hold them.
-template <class T, int V, bool OWN> Status ln_backward_fit(LnArgs &a, cudaStream_t st) {
+template <class T, int V, int NP, int D, int MAXT, int CTAS, int MODE>
+Status ln_backward_held(LnArgs &a, int G, int block, cudaStream_t st) {
+    if (MODE == kLnOwn && a.cols == (LL) G * NP * V) return ln_backward_rows<T, V, NP, D, MAXT, CTAS, MODE == kLnOwn ? kLnFull : MODE>(a, G, block, st);
+    return ln_backward_rows<T, V, NP, D, MAXT, CTAS, MODE>(a, G, block, st);
+}
+
+template <class T, int V, int MODE> Status ln_backward_fit(LnArgs &a, cudaStream_t st) {
     typedef LnFit<T> F;
-    constexpr int kStages = sizeof(T) == 2 ? 6 : 4;          // 192 KB per SM for float and double, 144 KB for half
-    if (int G = threads_for(a.cols, F::kSmall, 256)) return ln_backward_rows<T, V, F::kSmall / V, kStages, 256, 3, OWN>(a, G, 256 / G * G, st);
-    if (int G = threads_for(a.cols, F::kSmall, 512)) return ln_backward_rows<T, V, F::kSmall / V, kStages, 512, 1, OWN>(a, G, G, st);
-    return ln_backward_rows<T, V, F::kMid / V, 3, 512, 1, OWN>(a, threads_for(a.cols, F::kMid, 512), threads_for(a.cols, F::kMid, 512), st);
+    constexpr int S = F::kBackward;
+    if (int G = threads_for(a.cols, S, 256)) return ln_backward_held<T, V, S / V, F::kBackwardStages, 256, F::kBackwardCtas, MODE>(a, G, 256 / G * G, st);
+    if (int G = threads_for(a.cols, S, 512)) return ln_backward_held<T, V, S / V, F::kBackwardStages, 512, 1, MODE>(a, G, G, st);
+    if constexpr (F::kBackwardTwice) {
+        const int G = threads_for(a.cols, 2 * S, 512);
+        return ln_backward_held<T, V, 2 * S / V, 3, 512, 1, MODE>(a, G, G, st);
+    }
+    return bad_arg("layer norm gradient: row too long for the registers");
 }
 
 template <class T> Status ln_backward(LnArgs &a, bool rows, bool words, cudaStream_t st) {
     typedef typename Elem<T>::C C;
-    if (rows && a.rows > 0 && threads_for(a.cols, LnFit<T>::kMid, 512)) {
-        if (words) return ln_backward_fit<T, Elem<T>::kVec, true>(a, st);
-        return ln_backward_fit<T, 1, sizeof(T) >= 4>(a, st);
-    }
+    if (rows && a.rows > 0 && threads_for(a.cols, LnFit<T>::kBackwardMost, 512))
+        return words ? ln_backward_fit<T, Elem<T>::kVec, kLnOwn>(a, st) : ln_backward_fit<T, LnFit<T>::kPick, kLnPicked>(a, st);
     Scratch scratch(st);
     if (a.dGain || a.dBias) {
         // before dx is written, which may take the place of x or dz
