@@ -29,6 +29,7 @@ struct LnArgs {
     void *partials;                  // backward: [CTA][2][cols] wide values
     void *dGain, *dBias;             // may be null
     int numPartials;
+    int statBytes;                   // backward: where the statistics of the staged rows begin in shared memory
     View xOuter, xInner, zOuter, zInner, dzOuter, dzInner;      // for the sweeping kernels
 };
 
@@ -136,6 +137,10 @@ enum LnMode { kLnPicked = 0, kLnOwn = 1, kLnFull = 2 };
 ND_D void ln_copy(void *to, const void *from) {
     const unsigned s = (unsigned) __cvta_generic_to_shared(to);
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(s), "l"(from) : "memory");
+}
+template <class C> ND_D void ln_copy_value(C *to, const C *from) {
+    const unsigned s = (unsigned) __cvta_generic_to_shared(to);
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(s), "l"(from), "n"(sizeof(C)) : "memory");
 }
 ND_D void ln_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> ND_D void ln_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -343,20 +348,27 @@ __global__ void __launch_bounds__(MAXT, CTAS) k_ln_backward(const LnArgs a, cons
     sb.zero();
     const LL step = (LL) gridDim.x * g.groups;
     LL r = (LL) blockIdx.x * g.groups + g.group;
+    // mean and invStd travel with their row, a copy for every warp, made by its first two lanes: loaded one row ahead into
+    // registers, they were what half rows waited for (32768 rows of 4096 halves: 212 us)
+    const int lane = threadIdx.x & 31;
+    C *stats = reinterpret_cast<C *>(ln_smem + a.statBytes) + (threadIdx.x >> 5) * 2;
+    auto stat = [&](int d) { return stats + d * (blockDim.x >> 5) * 2; };
     auto fetch = [&](int d, LL row) {
-        if (row < a.rows) { g.fetch(d, 0, px + row * a.xRow); g.fetch(d, 1, pdz + row * a.dzRow); }
+        if (row < a.rows) {
+            g.fetch(d, 0, px + row * a.xRow);
+            g.fetch(d, 1, pdz + row * a.dzRow);
+            if (lane < 2) ln_copy_value(stat(d) + lane, (lane == 0 ? pMean : pInv) + row);
+        }
         ln_commit();
     };
-    C mean = C(0), inv = C(0);
-    if (r < a.rows) { mean = pMean[r]; inv = pInv[r]; }
 #pragma unroll
     for (int d = 0; d < D; d++) fetch(d, r + d * step);
     int stage = 0;
     auto plus = [](const LnPair<C> &x, const LnPair<C> &y) { return LnPair<C>{x.a + y.a, x.b + y.b}; };
     for (int parity = 0; r < a.rows; r += step, parity ^= 1) {
-        C nextMean = C(0), nextInv = C(0);
-        if (r + step < a.rows) { nextMean = pMean[r + step]; nextInv = pInv[r + step]; }
         ln_wait<D - 1>();
+        __syncwarp();
+        const C mean = stat(stage)[0], inv = stat(stage)[1];
         if (!OWN) ln_group_barrier(g.group, G);                // everyone's copies of this row stand
         Vals h, d;
         g.read(stage, 0, px + r * a.xRow, w);
@@ -374,7 +386,8 @@ __global__ void __launch_bounds__(MAXT, CTAS) k_ln_backward(const LnArgs a, cons
             pa = P::add(pa, d.p[i]);
             pb = P::fma(d.p[i], h.p[i], pb);
         }
-        if (OWN) fetch(stage, r + D * step);                   // these words have been read
+        __syncwarp();                                          // the warp has read its statistics
+        if (OWN) fetch(stage, r + D * step);                   // and this thread these words
         LnPair<C> s = {ln_warp_sum(pa.sum()), ln_warp_sum(pb.sum())};
         s = ln_group_sum<MAXT / 32>(s, slots[parity], g.group, G, plus);
         if (!OWN) { if ((G >> 5) == 1) __syncwarp(); fetch(stage, r + D * step); }         // nobody reads this stage any more
@@ -385,7 +398,6 @@ __global__ void __launch_bounds__(MAXT, CTAS) k_ln_backward(const LnArgs a, cons
             d.to(w);
             g.store(pdx + r * a.zRow, w);
         }
-        mean = nextMean; inv = nextInv;
         stage = stage + 1 == D ? 0 : stage + 1;
     }
     ln_wait<0>();
@@ -550,7 +562,7 @@ template <class T> struct LnFit {
     static constexpr int kForwardStages = sizeof(T) == 2 ? 6 : 4;       // 144 .. 192 KB of rows per SM
     static constexpr int kBackward = sizeof(T) == 8 ? 4 : (sizeof(T) == 4 ? 8 : 16);
     static constexpr int kBackwardCtas = sizeof(T) == 2 ? 2 : 3;
-    static constexpr int kBackwardStages = sizeof(T) == 2 ? 5 : 4;
+    static constexpr int kBackwardStages = sizeof(T) == 2 ? 5 : (sizeof(T) == 4 ? 4 : 3);
     static constexpr bool kBackwardTwice = sizeof(T) > 2;               // 32 halves and their sums do not fit
     static constexpr int kBackwardMost = kBackwardTwice ? 2 * kBackward : kBackward;
     static constexpr int kPick = sizeof(T) == 2 ? 2 : 1;                // values per word of rows that are no whole words
@@ -594,6 +606,9 @@ Status ln_forward_held(const LnArgs &a, int G, int block, cudaStream_t st) {
 
 template <class T, int V, int MODE> Status ln_forward_fit(const LnArgs &a, cudaStream_t st) {
     constexpr int S = LnFit<T>::kForward, D = LnFit<T>::kForwardStages;
+    // rows that a warp holds with a quarter of the values (half: with one word): most of its instructions would be idle
+    constexpr int Q = S / 4 > Elem<T>::kVec ? S / 4 : Elem<T>::kVec;
+    if (a.cols <= 32 * Q) return ln_forward_held<T, V, Q / V, D, 256, 4, MODE>(a, 32, 256, st);
     if (int G = threads_for(a.cols, S, 256)) return ln_forward_held<T, V, S / V, D, 256, 3, MODE>(a, G, 256 / G * G, st);
     if (int G = threads_for(a.cols, S, 512)) return ln_forward_held<T, V, S / V, D, 512, 1, MODE>(a, G, G, st);
     const int G = threads_for(a.cols, 2 * S, 512);
@@ -615,7 +630,9 @@ Status ln_backward_rows(LnArgs &a, int G, int block, cudaStream_t st) {
     const int groups = block / G;
     const size_t stages = MODE != kLnPicked ? (size_t) D * 2 * NP * V * sizeof(T) * block : (size_t) D * 2 * groups * ln_staged(a.cols, sizeof(T));
     const size_t fold = groups > 1 ? 2 * (size_t) a.cols * sizeof(C) : 0;
-    const size_t smem = stages > fold ? stages : fold;
+    const size_t rowsAndStats = stages + (size_t) D * 2 * (block / 32) * sizeof(C);
+    const size_t smem = rowsAndStats > fold ? rowsAndStats : fold;
+    a.statBytes = (int) stages;
     auto kernel = k_ln_backward<T, V, NP, D, MAXT, CTAS, MODE>;
     if (smem > 48 * 1024 - 512) ND_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem));
     LL grid = (LL) kNumSMs * CTAS;
