@@ -13,8 +13,11 @@
 //
 // Rows that do not fit (long, or not of unit stride) take the sweeping kernels at the end of the file.
 #include "../../include/nd4j_b200.h"
+#include <cooperative_groups.h>
 #include "device_utils.cuh"
 #include "entry_checks.h"
+
+namespace cg = cooperative_groups;
 
 namespace nd4jb200 {
 namespace {
@@ -29,6 +32,8 @@ struct LnArgs {
     void *partials;                  // backward: [CTA][2][cols] wide values
     void *dGain, *dBias;             // may be null
     int numPartials;
+    int cluster;                     // rows split over the CTAs of a cluster: their number, and the columns of each
+    int splitCols;
     int statBytes;                   // backward: where the statistics of the staged rows begin in shared memory
     View xOuter, xInner, zOuter, zInner, dzOuter, dzInner;      // for the sweeping kernels
 };
@@ -249,9 +254,37 @@ template <int MAXW, class S, class ADD> ND_D S ln_group_sum(S v, S *slots, int g
     return r;
 }
 
+// Rows that one CTA cannot hold are split over the CTAs of a cluster, which join their sums through distributed shared
+// memory; without a split this CTA has the row to itself. `unit` counts clusters (or CTAs).
+template <bool SPLIT> struct LnPart {
+    int rank, unit, units, cols;
+    LL first;                        // column
+    ND_D LnPart(const LnArgs &a) : rank(0), unit(blockIdx.x), units(gridDim.x), cols((int) a.cols), first(0) {
+        if constexpr (SPLIT) {
+            rank = (int) cg::this_cluster().block_rank();
+            unit = blockIdx.x / a.cluster;
+            units = gridDim.x / a.cluster;
+            first = (LL) rank * a.splitCols;
+            cols = a.cols - first < a.splitCols ? (int) (a.cols - first) : a.splitCols;
+        }
+    }
+    // Sum over the cluster, in the order of the CTAs. `joint` is written again only after another join in between.
+    template <class S, class ADD> ND_D S join(const LnArgs &a, S v, S *joint, ADD add) const {
+        if constexpr (SPLIT) {
+            cg::cluster_group cl = cg::this_cluster();
+            if (threadIdx.x == 0) *joint = v;
+            cl.sync();
+            v = *cl.map_shared_rank(joint, 0);
+            for (int q = 1; q < a.cluster; q++) v = add(v, *cl.map_shared_rank(joint, q));
+        }
+        return v;
+    }
+    ND_D void leave() const { if constexpr (SPLIT) cg::this_cluster().sync(); }      // nobody reads this CTA's memory any more
+};
+
 // Forward: two sums per row, the second around the mean. The slots alternate over four sets, so that a set is written
 // again only two barriers after it was read.
-template <class T, int V, int NP, int D, int MAXT, int CTAS, int MODE>
+template <class T, int V, int NP, int D, int MAXT, int CTAS, int MODE, bool SPLIT>
 __global__ void __launch_bounds__(MAXT, CTAS) k_ln_forward(const LnArgs a, const int G) {
     grid_dependency_sync();
     typedef typename Elem<T>::C C;
@@ -260,21 +293,23 @@ __global__ void __launch_bounds__(MAXT, CTAS) k_ln_forward(const LnArgs a, const
     extern __shared__ __align__(16) unsigned char ln_smem[];
     __shared__ C slots[4][MAXT / 32];
     constexpr bool OWN = MODE != kLnPicked;
-    const LnGroup<T, V, NP, 1, MODE> g(ln_smem, G, a.cols);
-    const T *px = static_cast<const T *>(a.x);
-    T *pz = static_cast<T *>(a.z);
+    __shared__ C joint[4];
+    const LnPart<SPLIT> part(a);
+    const LnGroup<T, V, NP, 1, MODE> g(ln_smem, G, part.cols);
+    const T *px = static_cast<const T *>(a.x) + part.first;
+    T *pz = static_cast<T *>(a.z) + part.first;
     const C invN = C(1) / (C) a.cols;
     Vals gain, bias;
     LnWord<T, V> w[NP];
-    if (a.gain) { g.load(static_cast<const T *>(a.gain), w); gain.from(w, g.values()); }
-    if (a.bias) { g.load(static_cast<const T *>(a.bias), w); bias.from(w, g.values()); }
+    if (a.gain) { g.load(static_cast<const T *>(a.gain) + part.first, w); gain.from(w, g.values()); }
+    if (a.bias) { g.load(static_cast<const T *>(a.bias) + part.first, w); bias.from(w, g.values()); }
 #pragma unroll
     for (int i = 0; i < Vals::N; i++) {
         if (!a.gain) gain.p[i] = P::all(C(1));
         if (!a.bias) bias.p[i] = P::all(C(0));
     }
-    const LL step = (LL) gridDim.x * g.groups;
-    LL r = (LL) blockIdx.x * g.groups + g.group;
+    const LL step = (LL) part.units * g.groups;
+    LL r = (LL) part.unit * g.groups + g.group;
 #pragma unroll
     for (int d = 0; d < D; d++) { if (r + d * step < a.rows) g.fetch(d, 0, px + (r + d * step) * a.xRow); ln_commit(); }
     int stage = 0;
@@ -289,6 +324,7 @@ __global__ void __launch_bounds__(MAXT, CTAS) k_ln_forward(const LnArgs a, const
 #pragma unroll
         for (int i = 1; i < Vals::N; i++) s = P::add(s, v.p[i]);
         C sum = ln_group_sum<MAXT / 32>(ln_warp_sum(s.sum()), slots[parity], g.group, G, plus);
+        sum = part.join(a, sum, joint + parity, plus);
         if (!OWN && (G >> 5) == 1) __syncwarp();
         // the stage has been read (OWN: by this thread, which alone uses these words; otherwise by all: the barrier)
         if (r + D * step < a.rows) g.fetch(stage, 0, px + (r + D * step) * a.xRow);
@@ -304,8 +340,9 @@ __global__ void __launch_bounds__(MAXT, CTAS) k_ln_forward(const LnArgs a, const
             else if (some) { if constexpr (P::W == 2) { const P one = P::of(v.p[i].get(0), C(0)); s = P::fma(one, one, s); } }
         }
         sum = ln_group_sum<MAXT / 32>(ln_warp_sum(s.sum()), slots[parity + 1], g.group, G, plus);
+        sum = part.join(a, sum, joint + parity + 1, plus);
         const C inv = C(1) / sqrt(sum * invN + (C) a.epsilon);
-        if (g.t == 0) {
+        if (g.t == 0 && part.rank == 0) {
             if (a.mean) static_cast<C *>(a.mean)[r] = mean;
             if (a.invStd) static_cast<C *>(a.invStd)[r] = inv;
         }
@@ -317,13 +354,14 @@ __global__ void __launch_bounds__(MAXT, CTAS) k_ln_forward(const LnArgs a, const
         stage = stage + 1 == D ? 0 : stage + 1;
     }
     ln_wait<0>();
+    part.leave();
 }
 
 template <class C> struct LnPair { C a, b; };
 
 // Backward: each thread holds the same columns of every row it meets, and therefore their sums of dg and db; a group
 // waits once per row, on a barrier of its own.
-template <class T, int V, int NP, int D, int MAXT, int CTAS, int MODE>
+template <class T, int V, int NP, int D, int MAXT, int CTAS, int MODE, bool SPLIT>
 __global__ void __launch_bounds__(MAXT, CTAS) k_ln_backward(const LnArgs a, const int G) {
     grid_dependency_sync();
     typedef typename Elem<T>::C C;
@@ -332,22 +370,24 @@ __global__ void __launch_bounds__(MAXT, CTAS) k_ln_backward(const LnArgs a, cons
     extern __shared__ __align__(16) unsigned char ln_smem[];
     __shared__ LnPair<C> slots[2][MAXT / 32];
     constexpr bool OWN = MODE != kLnPicked;
-    const LnGroup<T, V, NP, 2, MODE> g(ln_smem, G, a.cols);
-    const T *px = static_cast<const T *>(a.x), *pdz = static_cast<const T *>(a.dz);
-    T *pdx = static_cast<T *>(a.z);
+    __shared__ LnPair<C> joint[2];
+    const LnPart<SPLIT> part(a);
+    const LnGroup<T, V, NP, 2, MODE> g(ln_smem, G, part.cols);
+    const T *px = static_cast<const T *>(a.x) + part.first, *pdz = static_cast<const T *>(a.dz) + part.first;
+    T *pdx = a.z ? static_cast<T *>(a.z) + part.first : nullptr;
     const C *pMean = static_cast<const C *>(a.mean), *pInv = static_cast<const C *>(a.invStd);
     const C invN = C(1) / (C) a.cols;
     Vals gain, sg, sb;
     LnWord<T, V> w[NP];
-    if (a.gain) { g.load(static_cast<const T *>(a.gain), w); gain.from(w, g.values()); }
+    if (a.gain) { g.load(static_cast<const T *>(a.gain) + part.first, w); gain.from(w, g.values()); }
     else {
 #pragma unroll
         for (int i = 0; i < Vals::N; i++) gain.p[i] = P::all(C(1));
     }
     sg.zero();
     sb.zero();
-    const LL step = (LL) gridDim.x * g.groups;
-    LL r = (LL) blockIdx.x * g.groups + g.group;
+    const LL step = (LL) part.units * g.groups;
+    LL r = (LL) part.unit * g.groups + g.group;
     // mean and invStd travel with their row, a copy for every warp, made by its first two lanes: loaded one row ahead into
     // registers, they were what half rows waited for (32768 rows of 4096 halves: 212 us)
     const int lane = threadIdx.x & 31;
@@ -390,6 +430,7 @@ __global__ void __launch_bounds__(MAXT, CTAS) k_ln_backward(const LnArgs a, cons
         if (OWN) fetch(stage, r + D * step);                   // and this thread these words
         LnPair<C> s = {ln_warp_sum(pa.sum()), ln_warp_sum(pb.sum())};
         s = ln_group_sum<MAXT / 32>(s, slots[parity], g.group, G, plus);
+        s = part.join(a, s, joint + parity, plus);
         if (!OWN) { if ((G >> 5) == 1) __syncwarp(); fetch(stage, r + D * step); }         // nobody reads this stage any more
         if (pdx) {
             const P ma = P::all(-s.a * invN), mb = P::all(-s.b * invN);
@@ -401,10 +442,11 @@ __global__ void __launch_bounds__(MAXT, CTAS) k_ln_backward(const LnArgs a, cons
         stage = stage + 1 == D ? 0 : stage + 1;
     }
     ln_wait<0>();
+    part.leave();
     if (!a.dGain && !a.dBias) return;
     // the CTA's groups add up in shared memory, one after the other, then the CTA's sums become a partial row
-    C *pg = static_cast<C *>(a.partials) + (LL) blockIdx.x * 2 * a.cols, *pb = pg + a.cols;
-    C *tg = reinterpret_cast<C *>(ln_smem), *tb = tg + a.cols;
+    C *pg = static_cast<C *>(a.partials) + (LL) part.unit * 2 * a.cols + part.first, *pb = pg + a.cols;
+    C *tg = reinterpret_cast<C *>(ln_smem), *tb = tg + part.cols;
     __syncthreads();                                           // the stages have been read by all groups
     for (int q = 0; q < g.groups; q++) {
         if (q == g.group) {
@@ -576,24 +618,37 @@ inline unsigned grid_for(LL n) { return (unsigned) (n < 0x7fffffffLL ? (n > 0 ? 
 template <class K> inline void launch_with_smem(K kernel, dim3 grid, dim3 block, size_t smem, cudaStream_t st, const LnArgs &a, int G) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid; cfg.blockDim = block; cfg.dynamicSmemBytes = smem; cfg.stream = st;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = g_tuning[kTuneOverlapLaunch] ? 1 : 0;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned) a.cluster; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
+    cfg.attrs = g_tuning[kTuneOverlapLaunch] ? attr : attr + 1;
+    cfg.numAttrs = (g_tuning[kTuneOverlapLaunch] ? 1 : 0) + (a.cluster > 1 ? 1 : 0);
     cudaLaunchKernelEx(&cfg, kernel, a, G);
     count_launch();
 }
 
-template <class T, int V, int NP, int D, int MAXT, int CTAS, int MODE>
+// Cluster and columns per CTA of rows that are longer than `most`; 1 for the others, 0 for those that 8 CTAs cannot hold.
+inline int ln_split(LnArgs &a, LL most) {
+    a.cluster = 1;
+    a.splitCols = 0;
+    if (a.cols <= most) return 1;
+    while (a.cluster < 8 && a.cluster * most < a.cols) a.cluster *= 2;
+    a.splitCols = (int) (ceil_div(ceil_div(a.cols, a.cluster), 8) * 8);        // whole words of every type
+    return a.cluster * most < a.cols ? 0 : a.cluster;
+}
+
+template <class T, int V, int NP, int D, int MAXT, int CTAS, int MODE, bool SPLIT = false>
 Status ln_forward_rows(const LnArgs &a, int G, int block, cudaStream_t st) {
     const int groups = block / G;
-    const size_t smem = MODE != kLnPicked ? (size_t) D * NP * V * sizeof(T) * block : (size_t) D * groups * ln_staged(a.cols, sizeof(T));
-    auto kernel = k_ln_forward<T, V, NP, D, MAXT, CTAS, MODE>;
-    if (smem > 48 * 1024 - 512) ND_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem));
-    LL grid = (LL) kNumSMs * CTAS;
-    if (grid > ceil_div(a.rows, groups)) grid = ceil_div(a.rows, groups);
-    launch_with_smem(kernel, dim3((unsigned) grid), dim3((unsigned) block), smem, st, a, G);
+    const LL cols = SPLIT ? a.splitCols : a.cols;
+    const size_t smem = MODE != kLnPicked ? (size_t) D * NP * V * sizeof(T) * block : (size_t) D * groups * ln_staged(cols, sizeof(T));
+    auto kernel = k_ln_forward<T, V, NP, D, MAXT, CTAS, MODE, SPLIT>;
+    if (smem > 48 * 1024 - 1024) ND_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem));
+    LL units = (LL) kNumSMs * CTAS / a.cluster;
+    if (units > ceil_div(a.rows, groups)) units = ceil_div(a.rows, groups);
+    launch_with_smem(kernel, dim3((unsigned) (units * a.cluster)), dim3((unsigned) block), smem, st, a, G);
     ND_CUDA(cudaGetLastError());
     return kOk;
 }
@@ -611,12 +666,13 @@ template <class T, int V, int MODE> Status ln_forward_fit(const LnArgs &a, cudaS
     if (a.cols <= 32 * Q) return ln_forward_held<T, V, Q / V, D, 256, 4, MODE>(a, 32, 256, st);
     if (int G = threads_for(a.cols, S, 256)) return ln_forward_held<T, V, S / V, D, 256, 3, MODE>(a, G, 256 / G * G, st);
     if (int G = threads_for(a.cols, S, 512)) return ln_forward_held<T, V, S / V, D, 512, 1, MODE>(a, G, G, st);
-    const int G = threads_for(a.cols, 2 * S, 512);
-    return ln_forward_held<T, V, 2 * S / V, 3, 512, 1, MODE>(a, G, G, st);
+    if (int G = threads_for(a.cols, 2 * S, 512)) return ln_forward_held<T, V, 2 * S / V, 3, 512, 1, MODE>(a, G, G, st);
+    const int G = threads_for(a.splitCols, 2 * S, 512);
+    return ln_forward_rows<T, V, 2 * S / V, 3, 512, 1, MODE, true>(a, G, G, st);
 }
 
 template <class T> Status ln_forward(LnArgs &a, bool rows, bool words, cudaStream_t st) {
-    if (rows && threads_for(a.cols, 2 * LnFit<T>::kForward, 512))
+    if (rows && ln_split(a, 2 * LnFit<T>::kForward * 512))
         return words ? ln_forward_fit<T, Elem<T>::kVec, kLnOwn>(a, st) : ln_forward_fit<T, LnFit<T>::kPick, kLnPicked>(a, st);
     launch_kernel(k_ln_forward_sweep<T>, dim3(grid_for(a.rows)), dim3(kLnSweepThreads), st, a);
     ND_CUDA(cudaGetLastError());
@@ -624,27 +680,28 @@ template <class T> Status ln_forward(LnArgs &a, bool rows, bool words, cudaStrea
 }
 
 // Launches the kernel for rows of unit stride: `block` threads in groups of G, D stages of rows in shared memory.
-template <class T, int V, int NP, int D, int MAXT, int CTAS, int MODE>
+template <class T, int V, int NP, int D, int MAXT, int CTAS, int MODE, bool SPLIT = false>
 Status ln_backward_rows(LnArgs &a, int G, int block, cudaStream_t st) {
     typedef typename Elem<T>::C C;
     const int groups = block / G;
-    const size_t stages = MODE != kLnPicked ? (size_t) D * 2 * NP * V * sizeof(T) * block : (size_t) D * 2 * groups * ln_staged(a.cols, sizeof(T));
-    const size_t fold = groups > 1 ? 2 * (size_t) a.cols * sizeof(C) : 0;
+    const LL cols = SPLIT ? a.splitCols : a.cols;
+    const size_t stages = MODE != kLnPicked ? (size_t) D * 2 * NP * V * sizeof(T) * block : (size_t) D * 2 * groups * ln_staged(cols, sizeof(T));
+    const size_t fold = groups > 1 ? 2 * (size_t) cols * sizeof(C) : 0;
     const size_t rowsAndStats = stages + (size_t) D * 2 * (block / 32) * sizeof(C);
     const size_t smem = rowsAndStats > fold ? rowsAndStats : fold;
     a.statBytes = (int) stages;
-    auto kernel = k_ln_backward<T, V, NP, D, MAXT, CTAS, MODE>;
-    if (smem > 48 * 1024 - 512) ND_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem));
-    LL grid = (LL) kNumSMs * CTAS;
-    if (grid > ceil_div(a.rows, groups)) grid = ceil_div(a.rows, groups);
-    a.numPartials = (int) grid;
+    auto kernel = k_ln_backward<T, V, NP, D, MAXT, CTAS, MODE, SPLIT>;
+    if (smem > 48 * 1024 - 1024) ND_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem));
+    LL units = (LL) kNumSMs * CTAS / a.cluster;
+    if (units > ceil_div(a.rows, groups)) units = ceil_div(a.rows, groups);
+    a.numPartials = (int) units;
     Scratch scratch(st);
     const bool weights = a.dGain || a.dBias;
     if (weights) {
-        ND_TRY(scratch.alloc((size_t) grid * 2 * (size_t) a.cols * sizeof(C)));
+        ND_TRY(scratch.alloc((size_t) units * 2 * (size_t) a.cols * sizeof(C)));
         a.partials = scratch.at<void>(0);
     }
-    launch_with_smem(kernel, dim3((unsigned) grid), dim3((unsigned) block), smem, st, a, G);
+    launch_with_smem(kernel, dim3((unsigned) (units * a.cluster)), dim3((unsigned) block), smem, st, a, G);
     if (weights) launch_kernel(k_ln_fold<T>, dim3((unsigned) ceil_div(a.cols, 32)), dim3(1024), st, a);
     ND_CUDA(cudaGetLastError());
     return kOk;
@@ -661,16 +718,17 @@ template <class T, int V, int MODE> Status ln_backward_fit(LnArgs &a, cudaStream
     constexpr int S = F::kBackward;
     if (int G = threads_for(a.cols, S, 256)) return ln_backward_held<T, V, S / V, F::kBackwardStages, 256, F::kBackwardCtas, MODE>(a, G, 256 / G * G, st);
     if (int G = threads_for(a.cols, S, 512)) return ln_backward_held<T, V, S / V, F::kBackwardStages, 512, 1, MODE>(a, G, G, st);
-    if constexpr (F::kBackwardTwice) {
-        const int G = threads_for(a.cols, 2 * S, 512);
-        return ln_backward_held<T, V, 2 * S / V, 3, 512, 1, MODE>(a, G, G, st);
+    constexpr int M = F::kBackwardMost, D = M > S ? 3 : F::kBackwardStages;
+    if constexpr (M > S) {
+        if (int G = threads_for(a.cols, M, 512)) return ln_backward_held<T, V, M / V, D, 512, 1, MODE>(a, G, G, st);
     }
-    return bad_arg("layer norm gradient: row too long for the registers");
+    const int G = threads_for(a.splitCols, M, 512);
+    return ln_backward_rows<T, V, M / V, D, 512, 1, MODE, true>(a, G, G, st);
 }
 
 template <class T> Status ln_backward(LnArgs &a, bool rows, bool words, cudaStream_t st) {
     typedef typename Elem<T>::C C;
-    if (rows && a.rows > 0 && threads_for(a.cols, LnFit<T>::kBackwardMost, 512))
+    if (rows && a.rows > 0 && ln_split(a, LnFit<T>::kBackwardMost * 512))
         return words ? ln_backward_fit<T, Elem<T>::kVec, kLnOwn>(a, st) : ln_backward_fit<T, LnFit<T>::kPick, kLnPicked>(a, st);
     Scratch scratch(st);
     if (a.dGain || a.dBias) {
