@@ -557,14 +557,20 @@ __global__ void __launch_bounds__(LT, lp_ctas<T>(LT)) k_token_log_probs(const Lp
 }
 
 // ---- gradient ----------------------------------------------------------------------------------------------------
-constexpr int kLpGradThreads = 256;
-constexpr int kLpGradWords = 4;              // words in flight per thread, all a CTA does
+// Reads a word, writes a word. What costs beside the traffic is the wait for a row's values before anything can be
+// computed, so small CTAs, many per SM, each with all its words in flight from the start (8192 rows of 50001 halves: 291 us
+// with 256 threads of 4 words that waited for the row's values first, 277 so; 4096 rows of 32768 floats with entropy:
+// 182, 176).
+constexpr int kLpGradThreads = 128;
+template <class T> constexpr int kLpGradWords = sizeof(T) == 2 ? 8 : 4;       // per thread
+template <class T> constexpr int kLpGradCtas = sizeof(T) == 2 ? 8 : 10;
 
 template <class T, int V, bool ENT>
-__global__ void __launch_bounds__(kLpGradThreads) k_token_log_probs_grad(const LpArgs a) {
+__global__ void __launch_bounds__(kLpGradThreads, kLpGradCtas<T>) k_token_log_probs_grad(const LpArgs a) {
     grid_dependency_sync();
     typedef LpMath<T> M;
     typedef typename M::C C;
+    constexpr int W = kLpGradWords<T>;
     const C c = (C) (a.scale * M::kUnit), unit = (C) M::kUnit, back = (C) (1.0 / M::kUnit);
     const LL units = a.rows * a.chunks;
     for (LL b = blockIdx.x; b < units; b += gridDim.x) {
@@ -572,6 +578,12 @@ __global__ void __launch_bounds__(kLpGradThreads) k_token_log_probs_grad(const L
         const int chunk = (int) (b - r * a.chunks);
         const LpRow<T, V> row(a, r);
         T *dx = static_cast<T *>(a.dx) + r * a.dRow;
+        // the words are asked for before the row's values are known, padding or not: the two waits become one
+        const int first = chunk * (kLpGradThreads * W) + threadIdx.x;
+        alignas(16) T v[W][V];
+#pragma unroll
+        for (int j = 0; j < W; j++)
+            if (first + j * kLpGradThreads < row.words) row.load(first + j * kLpGradThreads, v[j]);
         const LL token = a.tokens[r];
         const C m = static_cast<const C *>(a.rowMax)[r], logSum = static_cast<const C *>(a.logSum)[r];
         const C g = (C) a.scale * (a.gLogProbs ? static_cast<const C *>(a.gLogProbs)[r] : C(0));
@@ -585,16 +597,9 @@ __global__ void __launch_bounds__(kLpGradThreads) k_token_log_probs_grad(const L
             const C lp = M::dist(x, ref, c) - shift, p = lp_exp(lp);
             return ENT ? p * fma(B, lp_finite(lp), A) : p * A;
         };
-        const int first = chunk * (kLpGradThreads * kLpGradWords) + threadIdx.x;
-        alignas(16) T v[kLpGradWords][V];
-        if (!none) {
-#pragma unroll
-            for (int j = 0; j < kLpGradWords; j++)
-                if (first + j * kLpGradThreads < row.words) row.load(first + j * kLpGradThreads, v[j]);
-        }
         const bool aligned = V > 1 && (reinterpret_cast<unsigned long long>(dx + row.head) & 15) == 0;
 #pragma unroll
-        for (int j = 0; j < kLpGradWords; j++) {
+        for (int j = 0; j < W; j++) {
             const int w = first + j * kLpGradThreads;
             if (w >= row.words) break;
             const int i = row.index(w);
@@ -673,7 +678,7 @@ template <class T> Status lp_forward(LpArgs &a, cudaStream_t st) {
 template <class T> Status lp_gradient(LpArgs &a, cudaStream_t st) {
     constexpr int V = Elem<T>::kVec;
     const bool unit = a.col == 1 && a.dCol == 1;
-    a.chunks = (int) ceil_div(ceil_div(a.vocab, unit ? V : 1), (LL) kLpGradThreads * kLpGradWords);
+    a.chunks = (int) ceil_div(ceil_div(a.vocab, unit ? V : 1), (LL) kLpGradThreads * kLpGradWords<T>);
     const LL units = a.rows * a.chunks;
     const dim3 grid((unsigned) (units < 0x7fffffffLL ? units : 0x7fffffffLL));
     const dim3 block(kLpGradThreads);
