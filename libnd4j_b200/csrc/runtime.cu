@@ -140,7 +140,12 @@ Status Scratch::alloc(size_t bytes) {
             g_pools[device] = pool;
         } else pool = it->second;
     }
-    ND_CUDA(cudaMallocFromPoolAsync(&ptr, bytes, pool, stream));
+    const cudaError_t e = cudaMallocFromPoolAsync(&ptr, bytes, pool, stream);
+    if (e != cudaSuccess) {
+        ptr = nullptr;
+        cudaGetLastError();                    // reported here: the next call is not to find it
+        return cuda_fail(e, "cudaMallocFromPoolAsync(scratch)");
+    }
     return kOk;
 }
 
