@@ -501,7 +501,8 @@ template <class T> Status emb_lookup(EmbArgs &a, bool words, cudaStream_t st) {
 
 template <class T, int KPT> Status launch_order_cluster(const OrderArgs &o, unsigned grid, unsigned cluster, cudaStream_t st) {
     const size_t smem = o.passes > 1 ? 2 * sizeof(unsigned) * kOrdThreads * KPT : 0;
-    ND_CUDA(cudaFuncSetAttribute(k_order_cluster<T, KPT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem));
+    static std::atomic<unsigned long long> asked{0};
+    ND_TRY(allow_shared(reinterpret_cast<const void *>(k_order_cluster<T, KPT>), smem + sizeof(OrderShared), asked));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid); cfg.blockDim = dim3(kOrdThreads); cfg.dynamicSmemBytes = smem; cfg.stream = st;
     cudaLaunchAttribute attr[2];

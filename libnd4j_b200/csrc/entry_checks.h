@@ -36,6 +36,22 @@ private:
     cudaStream_t stream;
     void *ptr = nullptr;
 };
+// Lets a kernel use `bytes` of dynamic shared memory, asked for once per kernel and device (about a microsecond each time
+// otherwise). `asked` is the kernel's own word, one bit per device.
+inline Status allow_shared(const void *kernel, size_t bytes, std::atomic<unsigned long long> &asked) {
+    if (bytes <= 46 * 1024) return kOk;             // 48 KB with what the kernels declare statically
+    int device = 0;
+    ND_CUDA(cudaGetDevice(&device));
+    const unsigned long long bit = 1ull << (device & 63);
+    if (device < 64 && (asked.load(std::memory_order_relaxed) & bit)) return kOk;
+    int most = 0;
+    ND_CUDA(cudaDeviceGetAttribute(&most, cudaDevAttrMaxSharedMemoryPerBlockOptin, device));
+    cudaFuncAttributes attr;
+    ND_CUDA(cudaFuncGetAttributes(&attr, kernel));
+    ND_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most - (int) attr.sharedSizeBytes));
+    asked.fetch_or(bit, std::memory_order_relaxed);
+    return kOk;
+}
 inline size_t round_up(size_t n, size_t to) { return (n + to - 1) / to * to; }
 
 inline size_t size_of_dtype(int dtype) { return dtype == kF64 ? 8 : (dtype == kF16 ? 2 : 4); }

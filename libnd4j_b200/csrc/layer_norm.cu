@@ -457,7 +457,11 @@ __global__ void __launch_bounds__(MAXT, CTAS) k_ln_backward(const LnArgs a, cons
                     C vg = sg.p[at / P::W].get(at % P::W), vb = sb.p[at / P::W].get(at % P::W);
                     if (q > 0) { vg += tg[c]; vb += tb[c]; }
                     if (q + 1 < g.groups) { tg[c] = vg; tb[c] = vb; }
-                    else { pg[c] = vg; pb[c] = vb; }
+                    else if (part.units > 1) { pg[c] = vg; pb[c] = vb; }
+                    else {                                     // the only partial row is the result
+                        if (a.dGain) static_cast<T *>(a.dGain)[part.first + c] = Elem<T>::from_c(vg);
+                        if (a.dBias) static_cast<T *>(a.dBias)[part.first + c] = Elem<T>::from_c(vb);
+                    }
                 }
             }
         }
@@ -645,7 +649,8 @@ Status ln_forward_rows(const LnArgs &a, int G, int block, cudaStream_t st) {
     const LL cols = SPLIT ? a.splitCols : a.cols;
     const size_t smem = MODE != kLnPicked ? (size_t) D * NP * V * sizeof(T) * block : (size_t) D * groups * ln_staged(cols, sizeof(T));
     auto kernel = k_ln_forward<T, V, NP, D, MAXT, CTAS, MODE, SPLIT>;
-    if (smem > 48 * 1024 - 1024) ND_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem));
+    static std::atomic<unsigned long long> asked{0};
+    ND_TRY(allow_shared(reinterpret_cast<const void *>(kernel), smem, asked));
     LL units = (LL) kNumSMs * CTAS / a.cluster;
     if (units > ceil_div(a.rows, groups)) units = ceil_div(a.rows, groups);
     launch_with_smem(kernel, dim3((unsigned) (units * a.cluster)), dim3((unsigned) block), smem, st, a, G);
@@ -691,12 +696,13 @@ Status ln_backward_rows(LnArgs &a, int G, int block, cudaStream_t st) {
     const size_t smem = rowsAndStats > fold ? rowsAndStats : fold;
     a.statBytes = (int) stages;
     auto kernel = k_ln_backward<T, V, NP, D, MAXT, CTAS, MODE, SPLIT>;
-    if (smem > 48 * 1024 - 1024) ND_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem));
+    static std::atomic<unsigned long long> asked{0};
+    ND_TRY(allow_shared(reinterpret_cast<const void *>(kernel), smem, asked));
     LL units = (LL) kNumSMs * CTAS / a.cluster;
     if (units > ceil_div(a.rows, groups)) units = ceil_div(a.rows, groups);
     a.numPartials = (int) units;
     Scratch scratch(st);
-    const bool weights = a.dGain || a.dBias;
+    const bool weights = (a.dGain || a.dBias) && units > 1;
     if (weights) {
         ND_TRY(scratch.alloc((size_t) units * 2 * (size_t) a.cols * sizeof(C)));
         a.partials = scratch.at<void>(0);

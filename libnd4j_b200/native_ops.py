@@ -387,12 +387,20 @@ class NativeOps:
     @staticmethod
     def _kinds(dt):
         """torch's element types for a call: its own, the wide one, the one of tokens (None without torch)."""
-        if dt not in _torch_kinds:
+        kinds = _torch_kinds.get(dt)
+        if kinds is None:
             torch = sys.modules.get("torch")
             if torch is None or dt not in _KINDS:
                 return None, None, None
-            _torch_kinds[dt] = getattr(torch, _KINDS[dt]), getattr(torch, _WIDE[dt]), torch.int64
-        return _torch_kinds[dt]
+            kinds = _torch_kinds[dt] = getattr(torch, _KINDS[dt]), getattr(torch, _WIDE[dt]), torch.int64
+        return kinds
+
+    def _queue(self, extraPointers):
+        """The stream of a call, as ctypes takes it."""
+        if extraPointers is not None and len(extraPointers) > 1 and extraPointers[1]:
+            stream = extraPointers[1]
+            return stream if type(stream) is int else _ptr(stream)
+        return _ptr(self.stream)
 
     def _tensor(self, obj, name, device, kind=None, count=None):
         """Address of a device array. What a torch tensor tells about itself is checked: the device, the element
@@ -418,6 +426,8 @@ class NativeOps:
         p = self._tensor(obj, name, device, kind)
         if info and hasattr(obj, "get_device"):
             r = info[0]
+            if r == 2 and info[4] == 1 and info[3] == info[2] and obj.numel() == info[1] * info[2] and obj.is_contiguous():
+                return p                                # the usual case: a dense matrix
             low = high = 0
             for k in range(1, r + 1):
                 extent, stride = info[k], info[k + r]
@@ -457,12 +467,12 @@ class NativeOps:
         bias, mean and invStd may be None."""
         kind, wide, _ = self._kinds(dt)
         xsp, xl = _descriptor(xShapeInfo)
-        zsp, zl = _descriptor(zShapeInfo)
+        zsp, zl = (xsp, xl) if zShapeInfo is xShapeInfo else _descriptor(zShapeInfo)
         dims = list(dimension)[:dimensionLength]
         count, length = self._tads(xl, dims)
         device = self.lib.nd4jb200_get_device()
         self._check(self.lib.nd4jb200_exec_layer_norm(
-            self._stream(extraPointers), dt, self._array(x, "x", device, kind, xl), xsp,
+            self._queue(extraPointers), dt, self._array(x, "x", device, kind, xl), xsp,
             self._tensor(gain, "gain", device, kind, length), self._tensor(bias, "bias", device, kind, length), epsilon,
             self._array(z, "z", device, kind, zl), zsp, self._tensor(mean, "mean", device, wide, count),
             self._tensor(invStd, "invStd", device, wide, count), array("i", dims).tobytes(), dimensionLength))
@@ -472,13 +482,13 @@ class NativeOps:
         """Gradients of execLayerNorm (nd4jb200_exec_layer_norm_grad). gain, dx, dGain and dBias may be None."""
         kind, wide, _ = self._kinds(dt)
         xsp, xl = _descriptor(xShapeInfo)
-        dsp, dl = _descriptor(dzShapeInfo)
-        osp, ol = _descriptor(dxShapeInfo)
+        dsp, dl = (xsp, xl) if dzShapeInfo is xShapeInfo else _descriptor(dzShapeInfo)
+        osp, ol = (xsp, xl) if dxShapeInfo is xShapeInfo else _descriptor(dxShapeInfo)
         dims = list(dimension)[:dimensionLength]
         count, length = self._tads(xl, dims)
         device = self.lib.nd4jb200_get_device()
         self._check(self.lib.nd4jb200_exec_layer_norm_grad(
-            self._stream(extraPointers), dt, self._array(x, "x", device, kind, xl), xsp,
+            self._queue(extraPointers), dt, self._array(x, "x", device, kind, xl), xsp,
             self._tensor(gain, "gain", device, kind, length), self._tensor(mean, "mean", device, wide, count),
             self._tensor(invStd, "invStd", device, wide, count), self._array(dz, "dz", device, kind, dl), dsp,
             self._array(dx, "dx", device, kind, ol), osp, self._tensor(dGain, "dGain", device, kind, length),
@@ -493,7 +503,7 @@ class NativeOps:
         rows = xl[1]
         device = self.lib.nd4jb200_get_device()
         self._check(self.lib.nd4jb200_exec_token_log_probs(
-            self._stream(extraPointers), dt, self._array(logits, "logits", device, kind, xl), xsp,
+            self._queue(extraPointers), dt, self._array(logits, "logits", device, kind, xl), xsp,
             self._tensor(tokens, "tokens", device, whole, rows), scale, self._tensor(logProbs, "logProbs", device, wide, rows),
             self._tensor(entropy, "entropy", device, wide, rows), self._tensor(rowMax, "rowMax", device, wide, rows),
             self._tensor(logSum, "logSum", device, wide, rows), k, self._tensor(topTokens, "topTokens", device, whole, rows * k),
@@ -505,11 +515,11 @@ class NativeOps:
         gLogProbs or gEntropy may be None."""
         kind, wide, whole = self._kinds(dt)
         xsp, xl = _descriptor(logitsShapeInfo)
-        osp, ol = _descriptor(dLogitsShapeInfo)
+        osp, ol = (xsp, xl) if dLogitsShapeInfo is logitsShapeInfo else _descriptor(dLogitsShapeInfo)
         rows = xl[1]
         device = self.lib.nd4jb200_get_device()
         self._check(self.lib.nd4jb200_exec_token_log_probs_grad(
-            self._stream(extraPointers), dt, self._array(logits, "logits", device, kind, xl), xsp,
+            self._queue(extraPointers), dt, self._array(logits, "logits", device, kind, xl), xsp,
             self._tensor(tokens, "tokens", device, whole, rows), scale, self._tensor(rowMax, "rowMax", device, wide, rows),
             self._tensor(logSum, "logSum", device, wide, rows), self._tensor(entropy, "entropy", device, wide, rows),
             self._tensor(gLogProbs, "gLogProbs", device, wide, rows), self._tensor(gEntropy, "gEntropy", device, wide, rows),
@@ -522,7 +532,7 @@ class NativeOps:
         zsp, zl = _descriptor(zShapeInfo)
         device = self.lib.nd4jb200_get_device()
         self._check(self.lib.nd4jb200_exec_embedding(
-            self._stream(extraPointers), dt, self._array(table, "table", device, kind, tl), tsp,
+            self._queue(extraPointers), dt, self._array(table, "table", device, kind, tl), tsp,
             self._tensor(tokens, "tokens", device, whole, zl[1]), scale, self._array(z, "z", device, kind, zl), zsp))
 
     def execEmbeddingGrad(self, dt, extraPointers, tokens, scale, dz, dzShapeInfo, grad, gradShapeInfo, accumulate=False):
@@ -532,7 +542,7 @@ class NativeOps:
         gsp, gl = _descriptor(gradShapeInfo)
         device = self.lib.nd4jb200_get_device()
         self._check(self.lib.nd4jb200_exec_embedding_grad(
-            self._stream(extraPointers), dt, self._tensor(tokens, "tokens", device, whole, dl[1]), scale,
+            self._queue(extraPointers), dt, self._tensor(tokens, "tokens", device, whole, dl[1]), scale,
             self._array(dz, "dz", device, kind, dl), dsp, self._array(grad, "grad", device, kind, gl), gsp,
             1 if accumulate else 0))
 
@@ -561,7 +571,7 @@ class NativeOps:
         if len(counts) < n:
             raise Nd4jError(1, "fewer lengths than tensors")
         device = self.lib.nd4jb200_get_device()
-        self._check(self.lib.nd4jb200_exec_global_norm(self._stream(extraPointers), dt,
+        self._check(self.lib.nd4jb200_exec_global_norm(self._queue(extraPointers), dt,
                                                        self._tensorList(x, "a tensor of x", device, kind, counts[:n]), lsp, n,
                                                        self._tensor(norm, "norm", device, wide, 1)))
 
@@ -574,7 +584,7 @@ class NativeOps:
             raise Nd4jError(1, "fewer lengths than tensors")
         device = self.lib.nd4jb200_get_device()
         zs = None if z is None else self._tensorList(z, "a tensor of z", device, kind, counts[:n])
-        self._check(self.lib.nd4jb200_exec_clip_by_global_norm(self._stream(extraPointers), dt,
+        self._check(self.lib.nd4jb200_exec_clip_by_global_norm(self._queue(extraPointers), dt,
                                                                self._tensorList(x, "a tensor of x", device, kind, counts[:n]), zs,
                                                                lsp, n, maxNorm, self._tensor(norm, "norm", device, wide, 1)))
 
