@@ -170,7 +170,7 @@ __global__ void __launch_bounds__(kGnThreads, kGnCtasPerSm) k_clip_by_norm(const
 // Few values: one launch of one cluster, which keeps them in registers between the two sweeps and joins its sums through
 // distributed shared memory (40 tensors of 200000 floats in all: 13.6 us in two launches, 11.6 so, from the start of a
 // replayed graph).
-constexpr int kGnOneThreads = 1024, kGnOneCtas = 8, kGnOneWords = 6;
+constexpr int kGnOneThreads = 1024, kGnOneCtas = 8, kGnOneWords = 8;
 constexpr LL kGnOneMost = (LL) kGnOneThreads * kGnOneCtas * kGnOneWords;        // words
 template <class T, bool SCALE>
 __global__ void __launch_bounds__(kGnOneThreads) k_clip_at_once(const __grid_constant__ GnArgs<kGnFewTensors> a) {
@@ -184,19 +184,19 @@ __global__ void __launch_bounds__(kGnOneThreads) k_clip_at_once(const __grid_con
     __syncthreads();
     Pack<T> v[kGnOneWords];
     int tensor[kGnOneWords];
-    LL at[kGnOneWords];
     double s = 0;
+    auto word = [&](int j) { return (j * kGnOneCtas + (int) blockIdx.x) * kGnOneThreads + (int) threadIdx.x; };
+    auto element = [&](int j, const GnTensor &t) { return (LL) (word(j) - t.firstChunk) * V - t.head; };
 #pragma unroll
     for (int j = 0; j < kGnOneWords; j++) {
-        const int w = (j * kGnOneCtas + (int) cl.block_rank()) * kGnOneThreads + threadIdx.x;
+        const int w = word(j);
         int lo = 0, hi = a.numTensors - 1;
         while (lo < hi) {
             const int mid = (lo + hi + 1) >> 1;
             if (table[mid].firstChunk <= w) lo = mid; else hi = mid - 1;
         }
         tensor[j] = w < a.numChunks ? lo : -1;                  // here the "chunks" are single words
-        at[j] = tensor[j] >= 0 ? (LL) (w - table[lo].firstChunk) * V - table[lo].head : 0;
-        if (tensor[j] >= 0) v[j] = gn_word(static_cast<const T *>(table[lo].x), at[j], table[lo].length, true);
+        if (tensor[j] >= 0) v[j] = gn_word(static_cast<const T *>(table[lo].x), element(j, table[lo]), table[lo].length, true);
     }
 #pragma unroll
     for (int j = 0; j < kGnOneWords; j++) if (tensor[j] >= 0) s += gn_square_sum<T>(v[j]);
@@ -224,7 +224,7 @@ __global__ void __launch_bounds__(kGnOneThreads) k_clip_at_once(const __grid_con
         const GnTensor &t = table[tensor[j]];
         if (!clip && t.x == t.z) continue;
         if (clip) gn_scale<T>(v[j], f);
-        gn_store<T>(static_cast<T *>(t.z), at[j], t.length, gn_words<T>(t), v[j]);
+        gn_store<T>(static_cast<T *>(t.z), element(j, t), t.length, gn_words<T>(t), v[j]);
     }
 }
 

@@ -110,14 +110,14 @@ template <class T, int V, int NP> struct LnVals {
 #pragma unroll
         for (int i = 0; i < N; i++) p[i] = P::all(C(0));
     }
-    template <class W> ND_D void from(const W (&w)[NP], int live, C beyond = C(0)) {      // `live`: values that exist
+    template <class W, class G> ND_D void from(const W (&w)[NP], const G &g, C beyond = C(0)) {
 #pragma unroll
         for (int i = 0; i < N; i++) {
             C e[P::W];
 #pragma unroll
             for (int k = 0; k < P::W; k++) {
                 const int at = i * P::W + k;
-                e[k] = at < live ? Elem<T>::to_c(w[at / V].v[at % V]) : beyond;
+                e[k] = g.exists(at) ? Elem<T>::to_c(w[at / V].v[at % V]) : beyond;
             }
             if constexpr (P::W == 2) p[i] = P::of(e[0], e[1]);
             else p[i] = P::all(e[0]);
@@ -137,8 +137,10 @@ template <class T, int V, int NP> struct LnVals {
 // element, what it shares with its neighbours' words), and every thread picks its columns from them behind a barrier;
 // half rows in pairs of columns, which are a 4-byte word in every second row of odd length. kLnFull: as kLnOwn, with every
 // word of every thread inside the row, so that no bounds are kept (forward, 16384 rows of 4096 floats: 28 instructions
-// per value with them).
-enum LnMode { kLnPicked = 0, kLnOwn = 1, kLnFull = 2 };
+// per value with them). kLn...Most: every word of a thread but its last one is, so that bounds are kept for that one.
+enum LnMode { kLnPicked = 0, kLnOwn = 1, kLnFull = 2, kLnPickedMost = 3, kLnOwnMost = 4 };
+ND_HD constexpr bool ln_own(int mode) { return mode == kLnOwn || mode == kLnFull || mode == kLnOwnMost; }
+ND_HD constexpr bool ln_most(int mode) { return mode == kLnPickedMost || mode == kLnOwnMost; }
 ND_D void ln_copy(void *to, const void *from) {
     const unsigned s = (unsigned) __cvta_generic_to_shared(to);
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(s), "l"(from) : "memory");
@@ -157,7 +159,8 @@ inline ND_HD int ln_staged(LL cols, int elem) { return (int) ((cols * elem + 15)
 // A CTA's groups of G threads, each holding one row at a time: thread t the words t, t + G, ... (NP at most) of V values.
 // The row's last word may be cut short: `live` counts the thread's values that exist, the first ones of its words.
 template <class T, int V, int NP, int NA, int MODE> struct LnGroup {
-    static constexpr bool OWN = MODE != kLnPicked, FULL = MODE == kLnFull;
+    static constexpr bool OWN = ln_own(MODE), FULL = MODE == kLnFull;
+    static constexpr int SURE = FULL ? NP : (ln_most(MODE) ? NP - 1 : 0);      // words that every thread has whole
     unsigned char *smem;
     int G, groups, group, t, have, live, staged;
     LL cols;
@@ -171,8 +174,8 @@ template <class T, int V, int NP, int NA, int MODE> struct LnGroup {
         if (have > 0 && word(have - 1) == words - 1) live -= words * V - (int) cols;
         staged = OWN ? 0 : ln_staged(cols, sizeof(T));
     }
-    ND_D int held() const { return FULL ? NP : have; }
-    ND_D int values() const { return FULL ? NP * V : live; }
+    ND_D bool holds(int j) const { return j < SURE || j < have; }
+    ND_D bool exists(int at) const { return at < SURE * V || at < live; }
     ND_D int word(int j) const { return t + G * j; }
     ND_D int column(int at) const { return word(at / V) * V + at % V; }
     // where stage d keeps word j of array q for this thread, or (not OWN) array q of this group
@@ -184,7 +187,7 @@ template <class T, int V, int NP, int NA, int MODE> struct LnGroup {
     ND_D void fetch(int d, int q, const T *row) const {
         if constexpr (OWN) {
 #pragma unroll
-            for (int j = 0; j < NP; j++) if (j < held()) ln_copy(own(d, q, j), row + word(j) * V);
+            for (int j = 0; j < NP; j++) if (holds(j)) ln_copy(own(d, q, j), row + word(j) * V);
         } else {
             const int off = shift(row), end = off + (int) cols * (int) sizeof(T), last = end / 16 * 16;
             const char *from = reinterpret_cast<const char *>(row) - off;
@@ -200,7 +203,7 @@ template <class T, int V, int NP, int NA, int MODE> struct LnGroup {
     ND_D void read(int d, int q, const T *row, LnWord<T, V> (&w)[NP]) const {
         if constexpr (OWN) {
 #pragma unroll
-            for (int j = 0; j < NP; j++) if (j < held()) w[j] = *own(d, q, j);
+            for (int j = 0; j < NP; j++) if (holds(j)) w[j] = *own(d, q, j);
         } else {
             const T *s = reinterpret_cast<const T *>(shared(d, q) + shift(row));
             pick(s, w);
@@ -211,32 +214,32 @@ template <class T, int V, int NP, int NA, int MODE> struct LnGroup {
     ND_D void pick(const T *p, LnWord<T, V> (&w)[NP]) const {
         if (V == 1 || (reinterpret_cast<unsigned long long>(p) & (sizeof(T) * V - 1)) == 0) {
 #pragma unroll
-            for (int j = 0; j < NP; j++) if (j < held()) w[j].load(p + word(j) * V);
+            for (int j = 0; j < NP; j++) if (holds(j)) w[j].load(p + word(j) * V);
         } else {
 #pragma unroll
             for (int j = 0; j < NP; j++)
 #pragma unroll
-                for (int k = 0; k < V; k++) if (j < held()) w[j].v[k] = p[word(j) * V + k];
+                for (int k = 0; k < V; k++) if (holds(j)) w[j].v[k] = p[word(j) * V + k];
         }
     }
     // The thread's values of a vector in global memory.
     ND_D void load(const T *p, LnWord<T, V> (&w)[NP]) const {
 #pragma unroll
-        for (int at = 0; at < NP * V; at++) if (at < values()) w[at / V].v[at % V] = p[column(at)];
+        for (int at = 0; at < NP * V; at++) if (exists(at)) w[at / V].v[at % V] = p[column(at)];
     }
     ND_D void store(T *p, const LnWord<T, V> (&w)[NP]) const {
         if (OWN || V == 1) {
 #pragma unroll
-            for (int j = 0; j < NP; j++) if (j < held()) w[j].store(p + word(j) * V);
+            for (int j = 0; j < NP; j++) if (holds(j)) w[j].store(p + word(j) * V);
         } else if ((reinterpret_cast<unsigned long long>(p) & (sizeof(T) * V - 1)) == 0) {
 #pragma unroll
             for (int j = 0; j < NP; j++) {
-                if (j * V + V <= values()) w[j].store(p + word(j) * V);
-                else if (j * V < values()) p[word(j) * V] = w[j].v[0];
+                if (exists(j * V + V - 1)) w[j].store(p + word(j) * V);
+                else if (exists(j * V)) p[word(j) * V] = w[j].v[0];
             }
         } else {
 #pragma unroll
-            for (int at = 0; at < NP * V; at++) if (at < values()) p[column(at)] = w[at / V].v[at % V];
+            for (int at = 0; at < NP * V; at++) if (exists(at)) p[column(at)] = w[at / V].v[at % V];
         }
     }
 };
@@ -292,7 +295,7 @@ __global__ void __launch_bounds__(MAXT, CTAS) k_ln_forward(const LnArgs a, const
     typedef LnVals<T, V, NP> Vals;
     extern __shared__ __align__(16) unsigned char ln_smem[];
     __shared__ C slots[4][MAXT / 32];
-    constexpr bool OWN = MODE != kLnPicked;
+    constexpr bool OWN = ln_own(MODE);
     __shared__ C joint[4];
     const LnPart<SPLIT> part(a);
     const LnGroup<T, V, NP, 1, MODE> g(ln_smem, G, part.cols);
@@ -301,8 +304,8 @@ __global__ void __launch_bounds__(MAXT, CTAS) k_ln_forward(const LnArgs a, const
     const C invN = C(1) / (C) a.cols;
     Vals gain, bias;
     LnWord<T, V> w[NP];
-    if (a.gain) { g.load(static_cast<const T *>(a.gain) + part.first, w); gain.from(w, g.values()); }
-    if (a.bias) { g.load(static_cast<const T *>(a.bias) + part.first, w); bias.from(w, g.values()); }
+    if (a.gain) { g.load(static_cast<const T *>(a.gain) + part.first, w); gain.from(w, g); }
+    if (a.bias) { g.load(static_cast<const T *>(a.bias) + part.first, w); bias.from(w, g); }
 #pragma unroll
     for (int i = 0; i < Vals::N; i++) {
         if (!a.gain) gain.p[i] = P::all(C(1));
@@ -319,7 +322,7 @@ __global__ void __launch_bounds__(MAXT, CTAS) k_ln_forward(const LnArgs a, const
         if (!OWN) ln_group_barrier(g.group, G);                // everyone's copies of this row stand
         g.read(stage, 0, px + r * a.xRow, w);
         Vals v;
-        v.from(w, g.values());
+        v.from(w, g);
         P s = v.p[0];
 #pragma unroll
         for (int i = 1; i < Vals::N; i++) s = P::add(s, v.p[i]);
@@ -335,7 +338,7 @@ __global__ void __launch_bounds__(MAXT, CTAS) k_ln_forward(const LnArgs a, const
 #pragma unroll
         for (int i = 0; i < Vals::N; i++) {
             v.p[i] = P::add(v.p[i], away);
-            const bool whole = i * P::W + P::W <= g.values(), some = i * P::W < g.values();
+            const bool whole = g.exists(i * P::W + P::W - 1), some = g.exists(i * P::W);
             if (whole) s = P::fma(v.p[i], v.p[i], s);
             else if (some) { if constexpr (P::W == 2) { const P one = P::of(v.p[i].get(0), C(0)); s = P::fma(one, one, s); } }
         }
@@ -369,7 +372,7 @@ __global__ void __launch_bounds__(MAXT, CTAS) k_ln_backward(const LnArgs a, cons
     typedef LnVals<T, V, NP> Vals;
     extern __shared__ __align__(16) unsigned char ln_smem[];
     __shared__ LnPair<C> slots[2][MAXT / 32];
-    constexpr bool OWN = MODE != kLnPicked;
+    constexpr bool OWN = ln_own(MODE);
     __shared__ LnPair<C> joint[2];
     const LnPart<SPLIT> part(a);
     const LnGroup<T, V, NP, 2, MODE> g(ln_smem, G, part.cols);
@@ -379,7 +382,7 @@ __global__ void __launch_bounds__(MAXT, CTAS) k_ln_backward(const LnArgs a, cons
     const C invN = C(1) / (C) a.cols;
     Vals gain, sg, sb;
     LnWord<T, V> w[NP];
-    if (a.gain) { g.load(static_cast<const T *>(a.gain) + part.first, w); gain.from(w, g.values()); }
+    if (a.gain) { g.load(static_cast<const T *>(a.gain) + part.first, w); gain.from(w, g); }
     else {
 #pragma unroll
         for (int i = 0; i < Vals::N; i++) gain.p[i] = P::all(C(1));
@@ -412,9 +415,9 @@ __global__ void __launch_bounds__(MAXT, CTAS) k_ln_backward(const LnArgs a, cons
         if (!OWN) ln_group_barrier(g.group, G);                // everyone's copies of this row stand
         Vals h, d;
         g.read(stage, 0, px + r * a.xRow, w);
-        h.from(w, g.values(), mean);                               // beyond the row: h = 0, dz = 0
+        h.from(w, g, mean);                               // beyond the row: h = 0, dz = 0
         g.read(stage, 1, pdz + r * a.dzRow, w);
-        d.from(w, g.values());
+        d.from(w, g);
         const P away = P::all(-mean), scale = P::all(inv);
         P pa = P::all(C(0)), pb = pa;
 #pragma unroll
@@ -452,7 +455,7 @@ __global__ void __launch_bounds__(MAXT, CTAS) k_ln_backward(const LnArgs a, cons
         if (q == g.group) {
 #pragma unroll
             for (int at = 0; at < NP * V; at++) {
-                if (at < g.values()) {
+                if (g.exists(at)) {
                     const int c = g.column(at);
                     C vg = sg.p[at / P::W].get(at % P::W), vb = sb.p[at / P::W].get(at % P::W);
                     if (q > 0) { vg += tg[c]; vb += tb[c]; }
@@ -647,7 +650,7 @@ template <class T, int V, int NP, int D, int MAXT, int CTAS, int MODE, bool SPLI
 Status ln_forward_rows(const LnArgs &a, int G, int block, cudaStream_t st) {
     const int groups = block / G;
     const LL cols = SPLIT ? a.splitCols : a.cols;
-    const size_t smem = MODE != kLnPicked ? (size_t) D * NP * V * sizeof(T) * block : (size_t) D * groups * ln_staged(cols, sizeof(T));
+    const size_t smem = ln_own(MODE) ? (size_t) D * NP * V * sizeof(T) * block : (size_t) D * groups * ln_staged(cols, sizeof(T));
     auto kernel = k_ln_forward<T, V, NP, D, MAXT, CTAS, MODE, SPLIT>;
     static std::atomic<unsigned long long> asked{0};
     ND_TRY(allow_shared(reinterpret_cast<const void *>(kernel), smem, asked));
@@ -661,6 +664,8 @@ Status ln_forward_rows(const LnArgs &a, int G, int block, cudaStream_t st) {
 template <class T, int V, int NP, int D, int MAXT, int CTAS, int MODE>
 Status ln_forward_held(const LnArgs &a, int G, int block, cudaStream_t st) {
     if (MODE == kLnOwn && a.cols == (LL) G * NP * V) return ln_forward_rows<T, V, NP, D, MAXT, CTAS, MODE == kLnOwn ? kLnFull : MODE>(a, G, block, st);
+    if (NP > 1 && a.cols / V >= (LL) G * (NP - 1))
+        return ln_forward_rows<T, V, NP, D, MAXT, CTAS, NP == 1 ? MODE : (MODE == kLnOwn ? kLnOwnMost : kLnPickedMost)>(a, G, block, st);
     return ln_forward_rows<T, V, NP, D, MAXT, CTAS, MODE>(a, G, block, st);
 }
 
@@ -690,7 +695,7 @@ Status ln_backward_rows(LnArgs &a, int G, int block, cudaStream_t st) {
     typedef typename Elem<T>::C C;
     const int groups = block / G;
     const LL cols = SPLIT ? a.splitCols : a.cols;
-    const size_t stages = MODE != kLnPicked ? (size_t) D * 2 * NP * V * sizeof(T) * block : (size_t) D * 2 * groups * ln_staged(cols, sizeof(T));
+    const size_t stages = ln_own(MODE) ? (size_t) D * 2 * NP * V * sizeof(T) * block : (size_t) D * 2 * groups * ln_staged(cols, sizeof(T));
     const size_t fold = groups > 1 ? 2 * (size_t) cols * sizeof(C) : 0;
     const size_t rowsAndStats = stages + (size_t) D * 2 * (block / 32) * sizeof(C);
     const size_t smem = rowsAndStats > fold ? rowsAndStats : fold;
@@ -716,6 +721,8 @@ Status ln_backward_rows(LnArgs &a, int G, int block, cudaStream_t st) {
 template <class T, int V, int NP, int D, int MAXT, int CTAS, int MODE>
 Status ln_backward_held(LnArgs &a, int G, int block, cudaStream_t st) {
     if (MODE == kLnOwn && a.cols == (LL) G * NP * V) return ln_backward_rows<T, V, NP, D, MAXT, CTAS, MODE == kLnOwn ? kLnFull : MODE>(a, G, block, st);
+    if (NP > 1 && a.cols / V >= (LL) G * (NP - 1))
+        return ln_backward_rows<T, V, NP, D, MAXT, CTAS, NP == 1 ? MODE : (MODE == kLnOwn ? kLnOwnMost : kLnPickedMost)>(a, G, block, st);
     return ln_backward_rows<T, V, NP, D, MAXT, CTAS, MODE>(a, G, block, st);
 }
 
