@@ -168,9 +168,9 @@ __global__ void __launch_bounds__(kGnThreads, kGnCtasPerSm) k_clip_by_norm(const
 }
 
 // Few values: one launch of one cluster, which keeps them in registers between the two sweeps and joins its sums through
-// distributed shared memory (40 tensors of 200000 floats in all: 13.6 us in two launches, 11.6 so, from the start of a
-// replayed graph).
-constexpr int kGnOneThreads = 1024, kGnOneCtas = 8, kGnOneWords = 8;
+// distributed shared memory. Two words per thread: 30000 floats take 8.2 us (10.9 in two launches, both from the start of
+// a replayed graph), 60000 10.3; with eight words 200000 floats take 14.3, since eight SMs then read what 54 would.
+constexpr int kGnOneThreads = 1024, kGnOneCtas = 8, kGnOneWords = 2;
 constexpr LL kGnOneMost = (LL) kGnOneThreads * kGnOneCtas * kGnOneWords;        // words
 template <class T, bool SCALE>
 __global__ void __launch_bounds__(kGnOneThreads) k_clip_at_once(const __grid_constant__ GnArgs<kGnFewTensors> a) {

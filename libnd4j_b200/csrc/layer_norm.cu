@@ -391,8 +391,11 @@ __global__ void __launch_bounds__(MAXT, CTAS) k_ln_backward(const LnArgs a, cons
     sb.zero();
     const LL step = (LL) part.units * g.groups;
     LL r = (LL) part.unit * g.groups + g.group;
-    // mean and invStd travel with their row, a copy for every warp, made by its first two lanes: loaded one row ahead into
-    // registers, they were what half rows waited for (32768 rows of 4096 halves: 212 us)
+    // Half: mean and invStd travel with their row, a copy for every warp, made by its first two lanes; loaded one row ahead
+    // into registers, they were what these shorter rows waited for (32768 rows of 4096 halves: 212 us, 153 so). Float and
+    // double rows last long enough for the load, and are better off without the two warp barriers (65536 rows of 1024
+    // floats: 141 us, 149 with them).
+    constexpr bool STAGED = sizeof(T) == 2;
     const int lane = threadIdx.x & 31;
     C *stats = reinterpret_cast<C *>(ln_smem + a.statBytes) + (threadIdx.x >> 5) * 2;
     auto stat = [&](int d) { return stats + d * (blockDim.x >> 5) * 2; };
@@ -400,18 +403,23 @@ __global__ void __launch_bounds__(MAXT, CTAS) k_ln_backward(const LnArgs a, cons
         if (row < a.rows) {
             g.fetch(d, 0, px + row * a.xRow);
             g.fetch(d, 1, pdz + row * a.dzRow);
-            if (lane < 2) ln_copy_value(stat(d) + lane, (lane == 0 ? pMean : pInv) + row);
+            if (STAGED && lane < 2) ln_copy_value(stat(d) + lane, (lane == 0 ? pMean : pInv) + row);
         }
         ln_commit();
     };
 #pragma unroll
     for (int d = 0; d < D; d++) fetch(d, r + d * step);
+    C mean = C(0), inv = C(0), nextMean = C(0), nextInv = C(0);
+    if (!STAGED && r < a.rows) { nextMean = pMean[r]; nextInv = pInv[r]; }
     int stage = 0;
     auto plus = [](const LnPair<C> &x, const LnPair<C> &y) { return LnPair<C>{x.a + y.a, x.b + y.b}; };
     for (int parity = 0; r < a.rows; r += step, parity ^= 1) {
+        if (!STAGED) {
+            mean = nextMean; inv = nextInv;
+            if (r + step < a.rows) { nextMean = pMean[r + step]; nextInv = pInv[r + step]; }
+        }
         ln_wait<D - 1>();
-        __syncwarp();
-        const C mean = stat(stage)[0], inv = stat(stage)[1];
+        if (STAGED) { __syncwarp(); mean = stat(stage)[0]; inv = stat(stage)[1]; }
         if (!OWN) ln_group_barrier(g.group, G);                // everyone's copies of this row stand
         Vals h, d;
         g.read(stage, 0, px + r * a.xRow, w);
@@ -429,7 +437,7 @@ __global__ void __launch_bounds__(MAXT, CTAS) k_ln_backward(const LnArgs a, cons
             pa = P::add(pa, d.p[i]);
             pb = P::fma(d.p[i], h.p[i], pb);
         }
-        __syncwarp();                                          // the warp has read its statistics
+        if (STAGED) __syncwarp();                              // the warp has read its statistics
         if (OWN) fetch(stage, r + D * step);                   // and this thread these words
         LnPair<C> s = {ln_warp_sum(pa.sum()), ln_warp_sum(pb.sum())};
         s = ln_group_sum<MAXT / 32>(s, slots[parity], g.group, G, plus);
