@@ -123,12 +123,17 @@ ND_D void order_rank(const unsigned (&key)[KPT], unsigned (&rank)[KPT], int shif
     __syncthreads();
 }
 
-// One element of T that is zero in every type.
+// Zeroes the table's rows; `first` and `step` deal the work to the threads (at least 16 of them).
 template <class T> ND_D void zero_rows(const OrderArgs &a, LL first, LL step) {
     T *z = static_cast<T *>(a.zero);
-    if (a.zeroWords > 0 && a.zeroRow == a.cols) {              // one run
-        const LL words = a.zeroRows * a.zeroWords;
-        uint4 *p = reinterpret_cast<uint4 *>(z);
+    if (a.zeroCol == 1 && a.zeroRow == a.cols) {                // one run: whole words but for its two ends
+        const LL n = a.zeroRows * a.cols;
+        LL head = (LL) (((16 - (reinterpret_cast<unsigned long long>(z) & 15)) & 15) / sizeof(T));
+        if (head > n) head = n;
+        const LL words = (n - head) / Elem<T>::kVec, tail = n - head - words * Elem<T>::kVec;
+        uint4 *p = reinterpret_cast<uint4 *>(z + head);
+        if (first < head) z[first] = Elem<T>::from_c(0);
+        if (first < tail) z[n - tail + first] = Elem<T>::from_c(0);
         LL i = first;
         for (; i + 3 * step < words; i += 4 * step) {
 #pragma unroll
