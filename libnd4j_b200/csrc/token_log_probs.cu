@@ -8,7 +8,8 @@
 // LogSoftMax followed by a gather writes the whole matrix to pick one value of each row, and an entropy takes three
 // more sweeps. Here a row is read once, as fast as HBM delivers it, each thread carrying the running maximum of what it
 // has seen and the two sums relative to it, rescaled in the rare step that moves the maximum; nothing but the results
-// is written. Sums are held in float for float and half data, in double for double.
+// is written. Sums are held in float for float and half data, in double for double. Measured: 4096 rows of 32768 floats,
+// 84 us = 6.4 TB/s (HBM); 8192 rows of 50001 halves, 147 us = 5.6 TB/s (HBM and, at 0.7, the exponentials).
 //
 // Exponentials are powers of two (one special-function instruction), so c carries the factor log2(e). Half data: the
 // distance from the reference point is one fused multiply-add, x c - R; R is the rounded m c, and since every term is
