@@ -335,8 +335,8 @@ int nd4jb200_exec_layer_norm_grad(void *stream, int dtype, const void *x, const 
 /* exec_token_log_probs: for every row x of the rank-2 logits, with p = softmax(scale * x): logProbs = log p[token],
  * entropy = -sum p log p, rowMax = max x, logSum = log sum exp(scale * (x - rowMax)), and the k best entries (larger
  * first, equal ones by index; a NaN before all) with their log probabilities, [rows, k] dense. k is at most 64 and at
- * most the row's length; scale is positive. Each of the wide results may be NULL; tokens (device, one per row) may be
- * NULL when logProbs is. A negative token marks padding: its row is not read and gives zeros and best tokens of -1. A
+ * most the row's length (0: topTokens and topLogProbs may be NULL); scale is positive. Each of the four per-row results may
+ * be NULL; tokens (device, one per row) may be NULL when logProbs is. A negative token marks padding: its row is not read and gives zeros and best tokens of -1. A
  * token at or beyond the row's length gives a NaN. Entries of -inf have probability 0; a row of nothing else gives log
  * probability -inf and entropy 0, a row with a NaN or +inf gives NaN.
  * exec_token_log_probs_grad: dLogits of  sum gLogProbs * logProbs + gEntropy * entropy  (one of the two may be NULL;

@@ -170,3 +170,61 @@ def test_rows_of_padding_cost_no_memory_access_and_leave_zeros(ops):
     dx = torch.full_like(x, 9.0)
     ops.execTokenLogProbsGrad(0, None, x, info(x), tokens, 1.0, out[2], out[3], out[1], g, g, dx, info(dx))
     assert (dx[[2, 4]] == 0).all() and dx[[0, 1, 3, 5]].isfinite().all()
+
+
+def test_ranks_repeated_dimensions_and_broadcast_rows(ops):
+    # a vector as one TAD; an axis named twice; an operand whose rows are all the same memory
+    x = randn(1, 5000).float()
+    z = torch.empty_like(x)
+    one = S.shape_info([5000])
+    mean, inv = torch.empty(1, device="cuda"), torch.empty(1, device="cuda")
+    ops.execLayerNorm(0, None, x, one, None, None, 1e-5, z, one, mean, inv, [0], 1)
+    w = x.double()
+    want = (w - w.mean()) / torch.sqrt(w.var(correction=0) + 1e-5)
+    within(z, want, 200 * U[0] * (want.abs() + 1))
+    x = randn(2, 7, 640).float()
+    a, b = torch.empty_like(x), torch.empty_like(x)
+    ops.execLayerNorm(0, None, x, info(x), None, None, 1e-5, a, info(a), None, None, [1], 1)
+    ops.execLayerNorm(0, None, x, info(x), None, None, 1e-5, b, info(b), None, None, [1, -1, 1], 3)
+    assert torch.equal(a, b)
+    same = S.shape_info([7, 640], "c", [0, 1], -1)
+    ops.execLayerNorm(0, None, x[0], same, None, None, 1e-5, b, info(b), None, None, [1], 1)
+    assert all(torch.equal(b[r], a[0]) for r in range(7))
+    tokens = torch.arange(7, device="cuda")
+    lp, full = torch.empty(7, device="cuda"), torch.empty(7, device="cuda")
+    ops.execTokenLogProbs(0, None, x[0], same, tokens, 1.0, lp, None, None, None)
+    ops.execTokenLogProbs(0, None, x[:1].expand(7, 640).contiguous(), info(x), tokens, 1.0, full, None, None, None)
+    assert torch.equal(lp, full)
+    grad = torch.empty(9, 640, device="cuda")
+    ops.execEmbeddingGrad(0, None, torch.full((7,), 3, dtype=torch.int64, device="cuda"), 1.0, x[0], same, grad, info(grad))
+    within(grad[3], 7 * x[0].double(), 10 * U[0] * 7 * x[0].double().abs())
+
+
+def test_launches_without_overlap(ops):
+    # programmatic launches switched off: the same bits
+    x, dz = randn(1, 900, 1024).float(), randn(2, 900, 1024).float()
+    gain, tokens = randn(3, 1024).float(), torch.randint(0, 50, (900,), device="cuda")
+    mean, inv = x.mean(1), 1 / torch.sqrt(x.var(1, correction=0) + 1e-5)
+
+    def run():
+        dx, dg, db = torch.empty_like(x), torch.empty_like(gain), torch.empty_like(gain)
+        grad, norm, lp = torch.empty(50, 1024, device="cuda"), torch.empty(1, device="cuda"), torch.empty(900, device="cuda")
+        ops.execLayerNormGrad(0, None, x, info(x), gain, mean, inv, dz, info(dz), dx, info(dx), dg, db, [1], 1)
+        ops.execEmbeddingGrad(0, None, tokens, 1.0, dx, info(dx), grad, info(grad))
+        ops.execTokenLogProbs(0, None, dx, info(dx), tokens, 1.0, lp, None, None, None)
+        ops.execClipByGlobalNorm(0, None, [grad, dg, db], None, [51200, 1024, 1024], 3, 0.5, norm)
+        ops.execClipByGlobalNorm(0, None, [dg], None, [1024], 1, 0.1, norm)
+        return dx, dg, db, grad, norm, lp
+    a = run()
+    ops._check(ops.lib.nd4jb200_set_tuning(3, 0))
+    try:
+        b = run()
+    finally:
+        ops._check(ops.lib.nd4jb200_set_tuning(3, 1))
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+def test_a_table_without_rows(ops):
+    table, z = torch.empty(0, 16, device="cuda"), torch.empty(3, 16, device="cuda")
+    ops.execEmbedding(0, None, table, info(table), torch.tensor([-1, 0, 5], device="cuda"), 1.0, z, info(z))
+    assert (z[0] == 0).all() and z[1:].isnan().all()
