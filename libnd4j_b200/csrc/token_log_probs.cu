@@ -11,9 +11,11 @@
 // is written. Sums are held in float for float and half data, in double for double. Measured: 4096 rows of 32768 floats,
 // 84 us = 6.4 TB/s (HBM); 8192 rows of 50001 halves, 147 us = 5.6 TB/s (HBM and, at 0.7, the exponentials).
 //
-// Exponentials are powers of two (one special-function instruction), so c carries the factor log2(e). Half data: the
-// distance from the reference point is one fused multiply-add, x c - R; R is the rounded m c, and since every term is
-// relative to the same R its rounding cancels exactly. Float data subtracts first: a value of the type's lowest, the
+// Exponentials are powers of two (one special-function instruction, relative error 2^-22), so c carries the factor log2(e).
+// Half data: the distance from the reference point is one fused multiply-add, x c - R. R is the rounded m c; every term is
+// relative to the same R, so its rounding cancels as long as it is a small exponent itself, which it is up to
+// 65504 c = 2^24 (half a unit in R's last place: 1/2). Larger scales, and float data at any, subtract first, (x - m) c: a
+// rounding of m c that passes 126 would leave nothing of the maximum's own term, and a float of the type's lowest value, the
 // usual mask, would overflow when multiplied. Masked entries (-inf) contribute nothing, a row of nothing else has log
 // probability -inf, entropy 0 and gradient 0; a row with a NaN or +inf answers NaN.
 //
@@ -48,9 +50,9 @@ constexpr int kLpList = 1024;               // collected candidates, at most
 constexpr int kLpNone = 0x7fffffff;
 
 // Exponent arithmetic of one element type. A reference point stands for a maximum; dist() is an element's exponent
-// relative to it, gap() that of another reference point.
-template <class T> struct LpMath;
-template <> struct LpMath<__half> {
+// relative to it, gap() that of another reference point. FAR: half data at a scale that its fused form does not serve.
+template <class T, bool FAR = false> struct LpMath;
+template <> struct LpMath<__half, false> {
     typedef float C;
     static constexpr float kFloor = -65504.f;       // reference of a row without values: the lowest finite one
     static constexpr double kUnit = 1.4426950408889634;          // log2(e): exponents are of base two
@@ -59,7 +61,7 @@ template <> struct LpMath<__half> {
     static ND_D float gap(float a, float b, float) { return a - b; }
     static ND_D float off(float m, float r, float c) { return fmaf(-m, c, r); }         // exponent of the reference over the maximum's
 };
-template <> struct LpMath<float> {
+template <> struct LpMath<float, false> {
     typedef float C;
     static constexpr float kFloor = -FLT_MAX;
     static constexpr double kUnit = 1.4426950408889634;
@@ -68,7 +70,8 @@ template <> struct LpMath<float> {
     static ND_D float gap(float a, float b, float c) { return (a - b) * c; }
     static ND_D float off(float, float, float) { return 0.f; }
 };
-template <> struct LpMath<double> {
+template <> struct LpMath<__half, true> : LpMath<float, false> {};
+template <> struct LpMath<double, false> {
     typedef double C;
     static constexpr double kFloor = -DBL_MAX;
     static constexpr double kUnit = 1.0;
@@ -164,10 +167,10 @@ template <class T, int V, int N> ND_D typename LpMath<T>::C lp_batch_max(const T
 
 // Moves sums from one reference point to another. A reference far below leaves a power of 0: its sum must not meet an
 // infinite gap.
-template <class T, bool ENT> ND_D void lp_move(typename LpMath<T>::C &s, typename LpMath<T>::C &u, typename LpMath<T>::C from,
-                                               typename LpMath<T>::C to, typename LpMath<T>::C c) {
-    typedef typename LpMath<T>::C C;
-    const C g = LpMath<T>::gap(from, to, c), f = lp_exp(g);
+template <class M, bool ENT> ND_D void lp_move(typename M::C &s, typename M::C &u, typename M::C from, typename M::C to,
+                                               typename M::C c) {
+    typedef typename M::C C;
+    const C g = M::gap(from, to, c), f = lp_exp(g);
     if (ENT) u = f == C(0) ? C(0) : f * fma(lp_finite(g), s, u);
     s *= f;
 }
@@ -354,10 +357,10 @@ ND_D void lp_select(const LpRow<T, V> &row, const LpKey<typename LpMath<T>::C> &
     __syncthreads();
 }
 
-template <class T, int V, bool ENT, bool TOP, int LT>
+template <class T, int V, bool ENT, bool TOP, int LT, bool FAR>
 __global__ void __launch_bounds__(LT, lp_ctas<T>(LT)) k_token_log_probs(const LpArgs a) {
     grid_dependency_sync();
-    typedef LpMath<T> M;
+    typedef LpMath<T, FAR> M;
     typedef typename M::C C;
     constexpr int kLpWarps = LT / 32;
     __shared__ LpShared<C, LT> s;
@@ -391,7 +394,7 @@ __global__ void __launch_bounds__(LT, lp_ctas<T>(LT)) k_token_log_probs(const Lp
         auto meet = [&](C bm, int where) {
             if (bm > top) {
                 const C to = M::ref(bm, c);
-                if (to > ref) { lp_move<T, ENT>(sum, sumU, ref, to, c); ref = to; }
+                if (to > ref) { lp_move<M, ENT>(sum, sumU, ref, to, c); ref = to; }
                 top = bm;
                 batch = where;
             }
@@ -443,7 +446,7 @@ __global__ void __launch_bounds__(LT, lp_ctas<T>(LT)) k_token_log_probs(const Lp
 #pragma unroll
         for (int w = 0; w < kLpWarps; w++) m = lp_max(m, s.tops[w]);
         LpSum<C> all = {M::ref(m, c), sum, sumU};
-        lp_move<T, ENT>(all.s, all.u, ref, all.ref, c);
+        lp_move<M, ENT>(all.s, all.u, ref, all.ref, c);
         for (int o = 16; o > 0; o >>= 1) {
             all.s += __shfl_xor_sync(0xffffffffu, all.s, o);
             if (ENT) all.u += __shfl_xor_sync(0xffffffffu, all.u, o);
@@ -472,7 +475,7 @@ __global__ void __launch_bounds__(LT, lp_ctas<T>(LT)) k_token_log_probs(const Lp
 #pragma unroll
             for (int q = 0; q < 8; q++) {
                 if (q < ctas) {
-                    lp_move<T, ENT>(qs[q], qu[q], M::ref(qm[q], c), all.ref, c);
+                    lp_move<M, ENT>(qs[q], qu[q], M::ref(qm[q], c), all.ref, c);
                     all.s += qs[q];
                     all.u += qu[q];
                 }
@@ -566,10 +569,10 @@ constexpr int kLpGradThreads = 128;
 template <class T> constexpr int kLpGradWords = sizeof(T) == 2 ? 8 : 4;       // per thread
 template <class T> constexpr int kLpGradCtas = sizeof(T) == 2 ? 8 : 10;
 
-template <class T, int V, bool ENT>
+template <class T, int V, bool ENT, bool FAR>
 __global__ void __launch_bounds__(kLpGradThreads, kLpGradCtas<T>) k_token_log_probs_grad(const LpArgs a) {
     grid_dependency_sync();
-    typedef LpMath<T> M;
+    typedef LpMath<T, FAR> M;
     typedef typename M::C C;
     constexpr int W = kLpGradWords<T>;
     const C c = (C) (a.scale * M::kUnit), unit = (C) M::kUnit, back = (C) (1.0 / M::kUnit);
@@ -646,17 +649,20 @@ template <class K> void launch_log_probs(K kernel, const LpArgs &a, unsigned gri
     count_launch();
 }
 
-template <class T, int V, int LT> void lp_forward_kernels(const LpArgs &a, unsigned grid, cudaStream_t st) {
+// Half data leaves the fused form once the rounding of the largest 65504 c exceeds half an exponent (scale above 177).
+bool lp_far(const LpArgs &a) { return a.scale * LpMath<__half>::kUnit * 65504.0 > 16777216.0; }
+
+template <class T, int V, int LT, bool FAR> void lp_forward_kernels(const LpArgs &a, unsigned grid, cudaStream_t st) {
     if (a.k > 0) {
-        if (a.entropy) launch_log_probs(k_token_log_probs<T, V, true, true, LT>, a, grid, LT, st);
-        else launch_log_probs(k_token_log_probs<T, V, false, true, LT>, a, grid, LT, st);
+        if (a.entropy) launch_log_probs(k_token_log_probs<T, V, true, true, LT, FAR>, a, grid, LT, st);
+        else launch_log_probs(k_token_log_probs<T, V, false, true, LT, FAR>, a, grid, LT, st);
     } else {
-        if (a.entropy) launch_log_probs(k_token_log_probs<T, V, true, false, LT>, a, grid, LT, st);
-        else launch_log_probs(k_token_log_probs<T, V, false, false, LT>, a, grid, LT, st);
+        if (a.entropy) launch_log_probs(k_token_log_probs<T, V, true, false, LT, FAR>, a, grid, LT, st);
+        else launch_log_probs(k_token_log_probs<T, V, false, false, LT, FAR>, a, grid, LT, st);
     }
 }
 
-template <class T> Status lp_forward(LpArgs &a, cudaStream_t st) {
+template <class T, bool FAR> Status lp_forward(LpArgs &a, cudaStream_t st) {
     constexpr int V = Elem<T>::kVec;
     // Rows that would leave SMs idle are shared by a cluster, as long as every CTA keeps at least one batch.
     a.cluster = 1;
@@ -667,16 +673,16 @@ template <class T> Status lp_forward(LpArgs &a, cudaStream_t st) {
     LL grid = a.rows * a.cluster;
     if (grid > 0x7fffffff / 8 * 8) grid = 0x7fffffff / 8 * 8;
     if (a.col == 1) {
-        if (shortRows) lp_forward_kernels<T, V, 32>(a, (unsigned) grid, st);
-        else lp_forward_kernels<T, V, kLpThreads>(a, (unsigned) grid, st);
+        if (shortRows) lp_forward_kernels<T, V, 32, FAR>(a, (unsigned) grid, st);
+        else lp_forward_kernels<T, V, kLpThreads, FAR>(a, (unsigned) grid, st);
     } else {
-        lp_forward_kernels<T, 1, kLpThreads>(a, (unsigned) grid, st);
+        lp_forward_kernels<T, 1, kLpThreads, FAR>(a, (unsigned) grid, st);
     }
     ND_CUDA(cudaGetLastError());
     return kOk;
 }
 
-template <class T> Status lp_gradient(LpArgs &a, cudaStream_t st) {
+template <class T, bool FAR> Status lp_gradient(LpArgs &a, cudaStream_t st) {
     constexpr int V = Elem<T>::kVec;
     const bool unit = a.col == 1 && a.dCol == 1;
     a.chunks = (int) ceil_div(ceil_div(a.vocab, unit ? V : 1), (LL) kLpGradThreads * kLpGradWords<T>);
@@ -684,11 +690,11 @@ template <class T> Status lp_gradient(LpArgs &a, cudaStream_t st) {
     const dim3 grid((unsigned) (units < 0x7fffffffLL ? units : 0x7fffffffLL));
     const dim3 block(kLpGradThreads);
     if (unit) {
-        if (a.gEntropy) launch_kernel(k_token_log_probs_grad<T, V, true>, grid, block, st, a);
-        else launch_kernel(k_token_log_probs_grad<T, V, false>, grid, block, st, a);
+        if (a.gEntropy) launch_kernel(k_token_log_probs_grad<T, V, true, FAR>, grid, block, st, a);
+        else launch_kernel(k_token_log_probs_grad<T, V, false, FAR>, grid, block, st, a);
     } else {
-        if (a.gEntropy) launch_kernel(k_token_log_probs_grad<T, 1, true>, grid, block, st, a);
-        else launch_kernel(k_token_log_probs_grad<T, 1, false>, grid, block, st, a);
+        if (a.gEntropy) launch_kernel(k_token_log_probs_grad<T, 1, true, FAR>, grid, block, st, a);
+        else launch_kernel(k_token_log_probs_grad<T, 1, false, FAR>, grid, block, st, a);
     }
     ND_CUDA(cudaGetLastError());
     return kOk;
@@ -704,7 +710,7 @@ Status lp_shape(const char *what, const ShapeDesc &d) {
     return kOk;
 }
 Status lp_scale(int dtype, double scale) {
-    // the exponent of the largest half, and of any difference that matters, has to stay a finite float
+    // the largest difference of two halves, times the scale, has to stay a finite float
     const double s = dtype == kF64 ? scale : (double) (float) scale;
     if (!(s > 0 && std::isfinite(s) && s <= 1e30)) return bad_arg("log probabilities: scale must be positive and at most 1e30");
     return kOk;
@@ -753,9 +759,9 @@ Status lp_forward_entry(void *stream, int dtype, const void *logits, const Nd4jL
     a.k = k; a.topTokens = topTokens; a.topLogProbs = topLogProbs;
     cudaStream_t cs = static_cast<cudaStream_t>(stream);
     switch (dtype) {
-        case kF32: return lp_forward<float>(a, cs);
-        case kF64: return lp_forward<double>(a, cs);
-        default: return lp_forward<__half>(a, cs);
+        case kF32: return lp_forward<float, false>(a, cs);
+        case kF64: return lp_forward<double, false>(a, cs);
+        default: return lp_far(a) ? lp_forward<__half, true>(a, cs) : lp_forward<__half, false>(a, cs);
     }
 }
 
@@ -797,9 +803,9 @@ Status lp_gradient_entry(void *stream, int dtype, const void *logits, const Nd4j
     a.dx = dLogits; a.dRow = o.stride[0]; a.dCol = o.shape[1] > 1 ? o.stride[1] : 1;
     cudaStream_t cs = static_cast<cudaStream_t>(stream);
     switch (dtype) {
-        case kF32: return lp_gradient<float>(a, cs);
-        case kF64: return lp_gradient<double>(a, cs);
-        default: return lp_gradient<__half>(a, cs);
+        case kF32: return lp_gradient<float, false>(a, cs);
+        case kF64: return lp_gradient<double, false>(a, cs);
+        default: return lp_far(a) ? lp_gradient<__half, true>(a, cs) : lp_gradient<__half, false>(a, cs);
     }
 }
 

@@ -270,3 +270,57 @@ def test_gradient_agrees_with_differences(ops):
         down = loss()
         x[at] = keep
         assert abs((up - down) / (2 * step) - float(dx[at])) < 1e-7
+
+
+def sharp_rows(dt, vocab):
+    """Rows for scales at which a row's maximum takes nearly all of it: maxima all over a logit's usual range, maxima that
+    two or three entries share, the largest half, masks."""
+    x = (randn(17, 12, vocab) * 4).to(KIND[dt])
+    x[1] = x[1] * 0.01 + 59.97
+    x[2, vocab // 3], x[2, vocab - 1] = 37.3125, 37.3125
+    x[3, 0], x[3, 1], x[3, vocab // 2] = 41.03125, 41.03125, 41.03125
+    x[4, 7] = 65504.0
+    x[5] = -65504.0
+    x[6, 3:] = -math.inf
+    x[7] = -math.inf
+    x[8] = x[8].abs() * -30 - 1
+    return x
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=NAMES.get)
+@pytest.mark.parametrize("scale", [170.0, 200.0, 1e6, 1e8, 1e29])
+@pytest.mark.parametrize("vocab", [64, 3001, 70000])
+def test_large_scales(ops, dt, scale, vocab):
+    x = sharp_rows(dt, vocab)
+    tokens = x.double().argmax(1)                         # log probabilities of nearly 0
+    tokens[9], tokens[10], tokens[11] = 1, -1, vocab
+    check(ops, dt, x, tokens, scale, 4)
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=NAMES.get)
+@pytest.mark.parametrize("scale", [170.0, 200.0, 1e6, 1e8, 1e29])
+@pytest.mark.parametrize("entropy_too", [False, True])
+def test_gradient_at_large_scales(ops, dt, scale, entropy_too):
+    # upstream gradients as small as the scale is large, so that the result stays in the range of a half
+    vocab = 3001
+    x = sharp_rows(dt, vocab)
+    rows = x.shape[0]
+    tokens = x.double().argmax(1)
+    tokens[9], tokens[10], tokens[11] = 1, -1, vocab
+    _, H, top, log_sum = truth(x, scale)
+    wide = [t.to(WIDE[dt]) for t in (top, log_sum, H)]
+    g = (randn(7, rows) / scale).to(WIDE[dt])
+    h = (randn(8, rows) / scale).to(WIDE[dt]) if entropy_too else None
+    want, log_p, entropy, p = grad_truth(x, tokens, scale, g.double(), None if h is None else h.double())
+    dx = torch.full_like(x, 5)
+    ops.execTokenLogProbsGrad(dt, None, x, info(x), tokens, scale, wide[0], wide[1], wide[2], g, h, dx, info(dx))
+    u = U[dt]
+    d = (log_p + log_sum[:, None]).abs()
+    rel = E[dt] + u * (8 * d + 6 * log_p.abs() + 8 * log_sum.abs()[:, None] + 8)
+    size = g.double().abs()[:, None] * p
+    if h is not None:
+        size = size + h.double().abs()[:, None] * p * (log_p.clamp(min=-1e4).abs() + entropy[:, None] + 1)
+    shared = torch.where(p > 0, size * (rel + 6 * u), 0)
+    # a probability below 2^-126 counts as 0 for float and half data: the shared part of it is below 2^-120
+    bound = scale * shared + 6 * u * scale * g.double().abs()[:, None] + STORE[dt] * want.abs() + TINY[dt]
+    within(dx, want, bound.nan_to_num(0, 0, 0))
