@@ -324,3 +324,42 @@ def test_gradient_at_large_scales(ops, dt, scale, entropy_too):
     # a probability below 2^-126 counts as 0 for float and half data: the shared part of it is below 2^-120
     bound = scale * shared + 6 * u * scale * g.double().abs()[:, None] + STORE[dt] * want.abs() + TINY[dt]
     within(dx, want, bound.nan_to_num(0, 0, 0))
+
+
+def collected(x, cluster, k, vec):
+    """How many candidates each CTA of a cluster collects for the k best of a row: the entries, at or above the k-th best of
+    its threads' maxima, of the slices whose maximum reaches it (a slice: every 256 * cluster-th word of 16 bytes)."""
+    words = x.double().view(-1, vec)
+    counts = []
+    for rank in range(cluster):
+        slices = [words[rank * 256 + t::256 * cluster].flatten() for t in range(256)]
+        tops = torch.stack([s.max() if s.numel() else torch.tensor(-math.inf, device=x.device, dtype=torch.float64) for s in slices])
+        least = tops.sort(descending=True).values[k - 1]
+        counts.append(sum(int((s >= least).sum()) for s, t in zip(slices, tops) if t >= least))
+    return counts
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=NAMES.get)
+@pytest.mark.parametrize("rows,vocab,cluster", [(160, 40000, 1), (3, 262144, 8)])
+def test_candidates_beyond_the_list(ops, dt, rows, vocab, cluster):
+    # the slices of nineteen threads lie above everything else, and those of a twentieth just below them: what reaches the
+    # twentieth's maximum is more than the 1024 candidates that are collected, and the best are then taken one by one
+    vec = 128 // torch.finfo(KIND[dt]).bits
+    x = randn(5, rows, vocab).to(KIND[dt])
+    span = 256 * cluster
+    words = x.view(rows, vocab // vec, vec)
+
+    def raise_slices(row, rank, first):
+        for t in range(20):
+            part = words[row, rank * 256 + first + t * 11::span]
+            steps = torch.arange(part.numel(), device="cuda").view(part.shape)
+            # distinct within a slice, in an order of their own, equal ones in other slices
+            part.copy_((16.0 if t == 7 else 32 + (steps * 37 % part.numel()) / 64.0) * torch.ones_like(steps, dtype=torch.float64))
+    raise_slices(0, 0, 3)
+    raise_slices(1, cluster - 1, 20)
+    for rank in range(cluster):
+        raise_slices(2, rank, rank)
+    x[2, 1] = 60000.0                                     # in the first of the raised slices
+    for row, where in ((0, 0), (1, cluster - 1), (2, 0)):
+        assert collected(x[row], cluster, 20, vec)[where] > 1024
+    check(ops, dt, x, some_tokens(rows, vocab), 1.0, 20)
