@@ -712,7 +712,7 @@ Status lp_shape(const char *what, const ShapeDesc &d) {
 Status lp_scale(int dtype, double scale) {
     // the largest difference of two halves, times the scale, has to stay a finite float
     const double s = dtype == kF64 ? scale : (double) (float) scale;
-    if (!(s > 0 && std::isfinite(s) && s <= 1e30)) return bad_arg("log probabilities: scale must be positive and at most 1e30");
+    if (!(s > 0 && scale <= 1e30)) return bad_arg("log probabilities: scale must be positive and at most 1e30");
     return kOk;
 }
 

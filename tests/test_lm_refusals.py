@@ -206,3 +206,12 @@ def test_the_mirror_checks_tensors(lib):
         ops.execLayerNorm(0, None, A, info, None, None, 1e-5, B, info, None, None, [5], 1)
     with pytest.raises(native_ops.Nd4jError, match="fewer"):
         ops.execGlobalNorm(0, None, [A, B], [3], 2, C)
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+def test_the_largest_scale_is_served(lib, dtype):
+    # (float) 1e30 is a little above 1e30; the limit is that of the number given. Without rows nothing is launched.
+    assert lib.nd4jb200_exec_token_log_probs(None, dtype, A, dense(0, 64), B, 1e30, C, None, None, None, 0, None, None) == 0
+    assert lib.nd4jb200_exec_token_log_probs_grad(None, dtype, A, dense(0, 64), B, 1e30, C, D, None, E, None, F, dense(0, 64)) == 0
+    refused(lib, lib.nd4jb200_exec_token_log_probs(None, dtype, A, dense(0, 64), B, np.nextafter(1e30, 2e30), C, None, None, None, 0, None,
+                                                   None), "scale")
