@@ -592,7 +592,8 @@ __global__ void __launch_bounds__(kLpGradThreads, kLpGradCtas<T>) k_token_log_pr
         const C m = static_cast<const C *>(a.rowMax)[r], logSum = static_cast<const C *>(a.logSum)[r];
         const C g = (C) a.scale * (a.gLogProbs ? static_cast<const C *>(a.gLogProbs)[r] : C(0));
         const C h = ENT ? (C) a.scale * static_cast<const C *>(a.gEntropy)[r] : C(0);
-        const bool none = token < 0 || m == -C(INFINITY);         // padding, or a row without a value: zeros
+        // padding, or a row without a value: zeros; a token beyond the row stays visible there too
+        const bool none = token < 0 || (m == -C(INFINITY) && token < a.vocab);
         const C ref = M::ref(m, c), shift = logSum * unit - M::off(m, ref, c);
         C A = ENT ? -(g + h * static_cast<const C *>(a.entropy)[r]) : -g;
         const C B = ENT ? -h * back : C(0);

@@ -363,3 +363,12 @@ def test_candidates_beyond_the_list(ops, dt, rows, vocab, cluster):
     for row, where in ((0, 0), (1, cluster - 1), (2, 0)):
         assert collected(x[row], cluster, 20, vec)[where] > 1024
     check(ops, dt, x, some_tokens(rows, vocab), 1.0, 20)
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=NAMES.get)
+@pytest.mark.parametrize("scale", [1.0, 500.0])
+@pytest.mark.parametrize("entropy_too", [False, True])
+def test_gradient_of_rows_without_values_for_tokens_beyond_them(ops, dt, scale, entropy_too):
+    x = (randn(9, 5, 333) * 2).to(KIND[dt])
+    x[:3] = -math.inf
+    check_grad(ops, dt, x, torch.tensor([333, 7, -1, 1000000, 5], device="cuda"), scale, entropy_too)
