@@ -113,9 +113,28 @@ template <class T> ND_D void gn_store(T *z, LL e, LL length, bool words, const P
         for (int k = 0; k < V; k++) if (e + k >= 0 && e + k < length) z[e + k] = v.v[k];
     }
 }
-template <class T> ND_D void gn_scale(Pack<T> &v, typename Elem<T>::C f) {
+// What the values are multiplied with. A factor near or below the type's smallest normal value would lose bits, or all of
+// them, that the products with values as large as such a norm still have: those are taken relative to the norm first, in double.
+template <class C> struct GnFactor {
+    C f;
+    bool clip, tiny;
+    double inv, most;
+    ND_D GnFactor(double n, double m) : inv(1.0 / n), most(m) {
+        clip = n > m && isfinite((C) n);
+        const double q = clip ? m / n : 1.0;
+        f = (C) q;
+        tiny = q < (sizeof(C) == 4 ? 0x1p-100 : 0x1p-1000) && m > 0;
+    }
+};
+template <class T> ND_D void gn_scale(Pack<T> &v, const GnFactor<typename Elem<T>::C> &g) {
+    typedef typename Elem<T>::C C;
+    if (!g.tiny) {
 #pragma unroll
-    for (int k = 0; k < Elem<T>::kVec; k++) v.v[k] = Elem<T>::from_c(Elem<T>::to_c(v.v[k]) * f);
+        for (int k = 0; k < Elem<T>::kVec; k++) v.v[k] = Elem<T>::from_c(Elem<T>::to_c(v.v[k]) * g.f);
+    } else {
+#pragma unroll
+        for (int k = 0; k < Elem<T>::kVec; k++) v.v[k] = Elem<T>::from_c((C) ((double) Elem<T>::to_c(v.v[k]) * g.inv * g.most));
+    }
 }
 template <class T> ND_D bool gn_words(const GnTensor &t) {          // z has x's place in a 16-byte word
     return ((reinterpret_cast<unsigned long long>(t.z) - (unsigned long long) t.head * sizeof(T)) & 15) == 0;
@@ -154,18 +173,17 @@ __global__ void __launch_bounds__(kGnThreads, kGnCtasPerSm) k_clip_by_norm(const
     const double norm = sqrt(gn_block_sum(s, slots));
     if (blockIdx.x == 0 && threadIdx.x == 0) *static_cast<C *>(a.norm) = (C) norm;
     if (!SCALE) return;
-    const bool clip = norm > a.maxNorm && isfinite((C) norm);
-    const C f = clip ? (C) (a.maxNorm / norm) : C(1);
+    const GnFactor<C> factor(norm, a.maxNorm);
     for (int c = a.numChunks - 1 - (int) blockIdx.x; c >= 0; c -= gridDim.x) {
         const GnTensor &t = a.t[gn_find(a, c)];
-        if (!clip && t.x == t.z) continue;
+        if (!factor.clip && t.x == t.z) continue;
         const LL firstWord = (LL) (c - t.firstChunk) * kGnChunk;
         Pack<T> v[kGnPacks];
         gn_load<T>(t, firstWord, false, v);
         const bool words = gn_words<T>(t);
 #pragma unroll
         for (int j = 0; j < kGnPacks; j++) {
-            if (clip) gn_scale<T>(v[j], f);
+            if (factor.clip) gn_scale<T>(v[j], factor);
             gn_store<T>(static_cast<T *>(t.z), (firstWord + (LL) j * kGnThreads + threadIdx.x) * V - t.head, t.length, words, v[j]);
         }
     }
@@ -220,14 +238,13 @@ __global__ void __launch_bounds__(kGnOneThreads) k_clip_at_once(const __grid_con
     const double norm = sqrt(s);
     if (blockIdx.x == 0 && threadIdx.x == 0) *static_cast<C *>(a.norm) = (C) norm;
     if (!SCALE) return;
-    const bool clip = norm > a.maxNorm && isfinite((C) norm);
-    const C f = clip ? (C) (a.maxNorm / norm) : C(1);
+    const GnFactor<C> factor(norm, a.maxNorm);
 #pragma unroll
     for (int j = 0; j < kGnOneWords; j++) {
         if (tensor[j] < 0) continue;
         const GnTensor &t = table[tensor[j]];
-        if (!clip && t.x == t.z) continue;
-        if (clip) gn_scale<T>(v[j], f);
+        if (!factor.clip && t.x == t.z) continue;
+        if (factor.clip) gn_scale<T>(v[j], factor);
         gn_store<T>(static_cast<T *>(t.z), element(j, t), t.length, gn_words<T>(t), v[j]);
     }
 }

@@ -109,3 +109,21 @@ def test_many_values_are_summed_the_same_way_each_time(ops):
     assert all(torch.equal(n, norms[0]) for n in norms)
     want = truth(x)
     within(norms[0][0], want, norm_bound(0, want))
+
+
+@pytest.mark.parametrize("dt,size,most", [(0, 1e34, 1e-6), (0, 1e35, 1e-25), (0, 1e30, 1e-30), (1, 1e150, 1e-170), (1, 1e140, 1e-150)])
+@pytest.mark.parametrize("lengths", [[900, 31], [200003, 17]])
+def test_factors_below_the_range_of_the_type(ops, dt, size, most, lengths):
+    # the factor maxNorm / norm has no (normal) value in the type; the products with the large values that need it do
+    x = tensors(dt, lengths, scale=size)
+    for t in x:
+        t[::3] *= 1e-3
+    norm = torch.empty(1, dtype=WIDE[dt], device="cuda")
+    want = truth(x)
+    z = [torch.full_like(t, 3) for t in x]
+    ops.execClipByGlobalNorm(dt, None, x, z, lengths, 2, most, norm)
+    within(norm[0], want, norm_bound(dt, want, 2))
+    for a, b in zip(x, z):
+        e = a.double() / want * most
+        slack = 0.5 * (240 + 2) + 2 if dt == 1 else 0           # of the norm itself, which is held in the type
+        within(b, e, e.abs() * ((10 + slack) * U[dt] + STORE[dt]) + TINY[dt])
