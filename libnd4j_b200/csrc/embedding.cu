@@ -301,7 +301,7 @@ struct EmbArgs {
     LL n, vocab, cols;
     LL srcRow, srcCol, dstRow, dstCol;
     double scale;
-    int words;                               // runs of V values per row
+    unsigned words;                          // runs of V values per row: below 2^31, so that a loop's last step still fits
     int group;                               // threads per row (a power of two from 8 to 256)
     // gradient
     const unsigned *key, *pos;
@@ -343,7 +343,7 @@ __global__ void __launch_bounds__(kEmbThreads, 6) k_embedding(const EmbArgs a) {
             row[r] = in[r] ? (int) token : 0;
             other[r] = token < 0 ? C(0) : (C) NAN;
         }
-        for (int w = t; w < a.words; w += a.group) {
+        for (unsigned w = t; w < a.words; w += a.group) {
             EmbWord<T, V> v[kEmbRows];
 #pragma unroll
             for (int r = 0; r < kEmbRows; r++)
@@ -360,7 +360,7 @@ __global__ void __launch_bounds__(kEmbThreads, 6) k_embedding(const EmbArgs a) {
 }
 
 // ---- gradient ----------------------------------------------------------------------------------------------------
-template <class T, int V, class C> ND_D void emb_finish(const EmbArgs &a, unsigned row, int w, const C (&sum)[V]) {
+template <class T, int V, class C> ND_D void emb_finish(const EmbArgs &a, unsigned row, unsigned w, const C (&sum)[V]) {
     T *g = static_cast<T *>(a.dst) + (LL) row * a.dstRow + (LL) w * V * a.dstCol;
     EmbWord<T, V> o;
     if (a.accumulate) o.load(g);
@@ -371,7 +371,7 @@ template <class T, int V, class C> ND_D void emb_finish(const EmbArgs &a, unsign
     }
     o.store(g);
 }
-template <int V, class C> ND_D void emb_partial(const EmbArgs &a, unsigned chunk, int which, int w, const C (&sum)[V]) {
+template <int V, class C> ND_D void emb_partial(const EmbArgs &a, unsigned chunk, int which, unsigned w, const C (&sum)[V]) {
     C *p = static_cast<C *>(a.partials) + ((LL) chunk * 2 + which) * a.cols + (LL) w * V;
 #pragma unroll
     for (int k = 0; k < V; k++) p[k] = sum[k];
@@ -398,7 +398,7 @@ __global__ void __launch_bounds__(kEmbThreads, 4) k_embedding_sums(const EmbArgs
     }
     __syncthreads();
     const T *dz = static_cast<const T *>(a.src);
-    for (int w = t + (int) blockIdx.y * a.group; w < a.words; w += a.group * (int) gridDim.y) {
+    for (unsigned w = t + blockIdx.y * a.group; w < a.words; w += a.group * gridDim.y) {
         C sum[V];
 #pragma unroll
         for (int k = 0; k < V; k++) sum[k] = C(0);
@@ -497,7 +497,7 @@ int group_for(LL words) {
 
 template <class T> Status emb_lookup(EmbArgs &a, bool words, cudaStream_t st) {
     constexpr int V = Elem<T>::kVec;
-    a.words = (int) (words ? a.cols / V : a.cols);
+    a.words = (unsigned) (words ? a.cols / V : a.cols);
     a.group = group_for(a.words);
     const LL blocks = ceil_div(a.n, (LL) kEmbThreads / a.group * kEmbRows);
     const dim3 grid((unsigned) (blocks < 0x7fffffffLL ? blocks : 0x7fffffffLL));
@@ -583,7 +583,7 @@ template <class T> Status emb_gradient(EmbArgs &a, OrderArgs &o, bool words, cud
         ND_CUDA(cudaGetLastError());
         return kOk;
     }
-    a.words = (int) (words ? a.cols / V : a.cols);
+    a.words = (unsigned) (words ? a.cols / V : a.cols);
     a.group = group_for(a.words);
     const LL slices = ceil_div(a.words, a.group);
     // Longer chunks mean fewer partial sums, shorter ones more CTAs: the longest of 8 .. 64 that still gives every SM

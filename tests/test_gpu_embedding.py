@@ -125,3 +125,17 @@ def test_lookup_and_gradient_are_transposed(ops):
     ops.execEmbeddingGrad(1, None, tokens, 2.5, dz, info(dz), grad, info(grad))
     a, b = float((z * dz).sum()), float((table * grad).sum())
     assert abs(a - b) < 1e-9
+
+
+def test_the_widest_rows(ops):
+    # 2^31 - 2 columns, no whole words: a loop's last step would pass 2^31
+    cols = 2 ** 31 - 2
+    table = torch.randint(-30000, 30000, (1, cols), device="cuda", dtype=torch.int16).view(torch.float16)
+    table[:, :] = table.nan_to_num(1.0, 1.0, 1.0)
+    token = torch.zeros(1, dtype=torch.int64, device="cuda")
+    z = torch.full((1, cols), 5.0, device="cuda", dtype=torch.float16)
+    ops.execEmbedding(2, None, table, info(table), token, 1.0, z, info(z))
+    assert torch.equal(z, table)
+    z.fill_(5.0)
+    ops.execEmbeddingGrad(2, None, token, 1.0, table, info(table), z, info(z))
+    assert torch.equal(z, table)

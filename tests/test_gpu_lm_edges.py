@@ -228,3 +228,25 @@ def test_a_table_without_rows(ops):
     table, z = torch.empty(0, 16, device="cuda"), torch.empty(3, 16, device="cuda")
     ops.execEmbedding(0, None, table, info(table), torch.tensor([-1, 0, 5], device="cuda"), 1.0, z, info(z))
     assert (z[0] == 0).all() and z[1:].isnan().all()
+
+
+def test_scratch_memory_goes_back_to_the_device(ops):
+    # 2^20 tokens of 4096 halves: 16384 chunks of the sorted list with two partial rows of floats each, 537 MB, besides 17 MB
+    # of lists. After a synchronisation no more than 128 MB of scratch memory may still be held.
+    n, cols = 1 << 20, 4096
+    dz = torch.ones(cols, device="cuda", dtype=torch.float16)
+    same = S.shape_info([n, cols], "c", [0, 1], -1)
+    tokens = torch.arange(n, device="cuda") % 7
+    grad = torch.empty(8, cols, device="cuda", dtype=torch.float16)
+    few = S.shape_info([100, cols], "c", [0, 1], -1)
+    ops.execEmbeddingGrad(2, None, tokens[:100], 2.0 ** -7, dz, few, grad, info(grad))          # loads what the calls need
+    big = torch.empty(5, device="cuda")
+    ops.execGlobalNorm(0, None, [big], [5], 1, torch.empty(1, device="cuda"))
+    torch.cuda.synchronize()
+    free = torch.cuda.mem_get_info()[0]
+    ops.execEmbeddingGrad(2, None, tokens, 2.0 ** -7, dz, same, grad, info(grad))
+    torch.cuda.synchronize()
+    held = free - torch.cuda.mem_get_info()[0]
+    counts = torch.bincount(tokens, minlength=8)
+    within(grad, (counts.double() / 128)[:, None].expand(8, cols), STORE[2] * (counts.double() / 128)[:, None] + TINY[2])
+    assert held <= (128 + 32) << 20, "%d MB are held" % (held >> 20)
