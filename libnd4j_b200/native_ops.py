@@ -445,6 +445,14 @@ class NativeOps:
         return p
 
     @staticmethod
+    def _axes(dimension, dimensionLength):
+        """The first dimensionLength entries of a dimension list."""
+        dims = list(dimension)
+        if not 0 <= dimensionLength <= len(dims):
+            raise Nd4jError(1, "the dimension list holds %d entries, not %d" % (len(dims), dimensionLength))
+        return dims[:dimensionLength]
+
+    @staticmethod
     def _tads(info, dimension):
         """Number of TADs of an array along a dimension list, and the length of one."""
         r = info[0]
@@ -468,7 +476,7 @@ class NativeOps:
         kind, wide, _ = self._kinds(dt)
         xsp, xl = _descriptor(xShapeInfo)
         zsp, zl = (xsp, xl) if zShapeInfo is xShapeInfo else _descriptor(zShapeInfo)
-        dims = list(dimension)[:dimensionLength]
+        dims = self._axes(dimension, dimensionLength)
         count, length = self._tads(xl, dims)
         device = self.lib.nd4jb200_get_device()
         self._check(self.lib.nd4jb200_exec_layer_norm(
@@ -484,7 +492,7 @@ class NativeOps:
         xsp, xl = _descriptor(xShapeInfo)
         dsp, dl = (xsp, xl) if dzShapeInfo is xShapeInfo else _descriptor(dzShapeInfo)
         osp, ol = (xsp, xl) if dxShapeInfo is xShapeInfo else _descriptor(dxShapeInfo)
-        dims = list(dimension)[:dimensionLength]
+        dims = self._axes(dimension, dimensionLength)
         count, length = self._tads(xl, dims)
         device = self.lib.nd4jb200_get_device()
         self._check(self.lib.nd4jb200_exec_layer_norm_grad(

@@ -215,3 +215,15 @@ def test_the_largest_scale_is_served(lib, dtype):
     assert lib.nd4jb200_exec_token_log_probs_grad(None, dtype, A, dense(0, 64), B, 1e30, C, D, None, E, None, F, dense(0, 64)) == 0
     refused(lib, lib.nd4jb200_exec_token_log_probs(None, dtype, A, dense(0, 64), B, np.nextafter(1e30, 2e30), C, None, None, None, 0, None,
                                                    None), "scale")
+
+
+def test_the_mirror_does_not_read_beyond_a_dimension_list(lib):
+    ops = native_ops.NativeOps()
+    info = S.shape_info([4, 8])
+    for dims, length in (([1], 2), ([], 1), ([1], 1 << 30), ([1], -1), (np.array([0, 1], dtype=np.int32), 3)):
+        with pytest.raises(native_ops.Nd4jError, match="dimension list holds"):
+            ops.execLayerNorm(0, None, A, info, None, None, 1e-5, B, info, None, None, dims, length)
+        with pytest.raises(native_ops.Nd4jError, match="dimension list holds"):
+            ops.execLayerNormGrad(0, None, A, info, None, B, C, D, info, E, info, None, None, dims, length)
+    with pytest.raises(native_ops.Nd4jError, match="dimension list is empty"):
+        ops.execLayerNorm(0, None, A, info, None, None, 1e-5, B, info, None, None, [1], 0)
