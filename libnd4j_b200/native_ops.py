@@ -68,6 +68,14 @@ def _ints(a):
     return arr, arr.ctypes.data_as(ctypes.POINTER(ctypes.c_int))
 
 
+def _dims(a, n):
+    """A dimension list of which a C function reads n entries."""
+    arr, p = _ints(a)
+    if arr is not None and arr.size < n:
+        raise Nd4jError(1, "the dimension list holds %d entries, not %d" % (arr.size, n))
+    return arr, p
+
+
 def _descriptor(a):
     """A shapeInfo (or another list of 64-bit integers) as the bytes that a C function reads, and as a list. (An array's
     own address costs ctypes ten times as much.)"""
@@ -222,7 +230,7 @@ class NativeOps:
                     dimension=None, dimensionLength=0):
         xs, xsp = _longs(xShapeInfo)
         zs, zsp = _longs(resultShapeInfo)
-        dm, dmp = _ints(dimension)
+        dm, dmp = _dims(dimension, dimensionLength)
         self._check(self.lib.nd4jb200_exec_reduce(self._stream(extraPointers), dt, opNum, _ptr(x), xsp,
                                                   _ptr(extraParams), _ptr(result), zsp, dmp, dimensionLength))
 
@@ -237,7 +245,7 @@ class NativeOps:
                          dimension=None, dimensionLength=0):
         xs, xsp = _longs(xShapeInfo)
         zs, zsp = _longs(resultShapeInfo)
-        dm, dmp = _ints(dimension)
+        dm, dmp = _dims(dimension, dimensionLength)
         self._check(self.lib.nd4jb200_exec_index_reduce(self._stream(extraPointers), dt, opNum, _ptr(x), xsp,
                                                         _ptr(extraParams), _ptr(result), zsp, dmp, dimensionLength))
 
@@ -255,7 +263,7 @@ class NativeOps:
             dimension, biasCorrected = None, dimension
         xs, xsp = _longs(xShapeInfo)
         zs, zsp = _longs(resultShapeInfo)
-        dm, dmp = _ints(dimension)
+        dm, dmp = _dims(dimension, dimensionLength)
         self._check(self.lib.nd4jb200_exec_summary_stats(self._stream(extraPointers), dt, opNum, _ptr(x), xsp,
                                                          _ptr(extraParams), _ptr(result), zsp, dmp, dimensionLength,
                                                          1 if biasCorrected else 0))
@@ -273,7 +281,7 @@ class NativeOps:
         xs, xsp = _longs(xShapeInfo)
         ys, ysp = _longs(yShapeInfo)
         zs, zsp = _longs(resultShapeInfo)
-        dm, dmp = _ints(dimension)
+        dm, dmp = _dims(dimension, dimensionLength)
         self._check(self.lib.nd4jb200_exec_reduce3(self._stream(extraPointers), dt, opNum, _ptr(x), xsp,
                                                    _ptr(extraParamsVals), _ptr(y), ysp, _ptr(result), zsp, dmp,
                                                    dimensionLength))
@@ -286,7 +294,7 @@ class NativeOps:
         xs, xsp = _longs(xInfo)
         ys, ysp = _longs(yInfo)
         zs, zsp = _longs(resultShapeInfoBuffer)
-        dm, dmp = _ints(dimension)
+        dm, dmp = _dims(dimension, dimensionLength)
         self._check(self.lib.nd4jb200_exec_reduce3_all(self._stream(extraPointers), dt, opNum, _ptr(x), xsp,
                                                        _ptr(extraParamsVals), _ptr(y), ysp, _ptr(result), zsp, dmp,
                                                        dimensionLength))
@@ -337,7 +345,7 @@ class NativeOps:
         xs, xsp = _longs(xShapeInfo)
         ys, ysp = _longs(yShapeInfo)
         zs, zsp = _longs(resultShapeInfo)
-        dm, dmp = _ints(dimension)
+        dm, dmp = _dims(dimension, dimensionLength)
         self._check(self.lib.nd4jb200_exec_broadcast(self._stream(extraPointers), dt, opNum, _ptr(x), xsp, _ptr(y), ysp,
                                                      _ptr(result), zsp, dmp, dimensionLength))
 
@@ -377,7 +385,7 @@ class NativeOps:
         bs, bsp = _longs(bShapeInfo)
         ys, ysp = _longs(yShapeInfo)
         zs, zsp = _longs(zShapeInfo)
-        dm, dmp = _ints(dimension)
+        dm, dmp = _dims(dimension, dimensionLength)
         self._check(self.lib.nd4jb200_exec_chain(self._stream(extraPointers), dt, broadcastOp, _ptr(x), xsp, _ptr(b), bsp,
                                                  dmp, dimensionLength, transformOp, _ptr(transformExtra), pairwiseOp,
                                                  _ptr(y), ysp, _ptr(pairwiseExtra), _ptr(z), zsp))
@@ -636,7 +644,7 @@ class NativeOps:
                                   dimension, dimensionLength):
         xs, xsp = _longs(xShapeInfo)
         zs, zsp = _longs(zShapeInfo)
-        dm, dmp = _ints(dimension)
+        dm, dmp = _dims(dimension, dimensionLength)
         self._check(self.lib.nd4jb200_exec_scalar_along_dimension(self._stream(extraPointers), dt, opNum, _ptr(x), xsp,
                                                                   _ptr(extraParams), _ptr(z), zsp, _ptr(scalars), dmp,
                                                                   dimensionLength))
@@ -708,7 +716,7 @@ class NativeOps:
     def tadOnlyShapeInfo(self, xShapeInfo, dimension, dimensionLength, target=None, offsets=None):
         """Returns (tadShapeInfo, tadOffsets) as numpy arrays (NativeOps.h:1880)."""
         xs, xsp = _longs(xShapeInfo)
-        dm, dmp = _ints(dimension)
+        dm, dmp = _dims(dimension, dimensionLength)
         n = self.lib.nd4jb200_tad_count(xsp, dmp, dimensionLength)
         if n < 0:
             raise Nd4jError(1, self.lastError())
@@ -840,7 +848,7 @@ class NativeOps:
     def _sortTad(self, dt, extraPointers, x, xShapeInfo, dimension, dimensionLength, tadShapeInfo=None, tadOffsets=None,
                  descending=False):
         xs, xsp = _longs(xShapeInfo)
-        d, dp = _ints(dimension)
+        d, dp = _dims(dimension, dimensionLength)
         self._check(self.lib.nd4jb200_sort_tad(self._stream(extraPointers), dt, _ptr(x), xsp, dp, dimensionLength,
                                                1 if descending else 0))
 

@@ -227,3 +227,18 @@ def test_the_mirror_does_not_read_beyond_a_dimension_list(lib):
             ops.execLayerNormGrad(0, None, A, info, None, B, C, D, info, E, info, None, None, dims, length)
     with pytest.raises(native_ops.Nd4jError, match="dimension list is empty"):
         ops.execLayerNorm(0, None, A, info, None, None, 1e-5, B, info, None, None, [1], 0)
+
+
+def test_the_other_members_do_not_read_beyond_a_dimension_list_either(lib):
+    ops = native_ops.NativeOps()
+    info, row = S.shape_info([4, 8]), S.shape_info([1, 8])
+    calls = (lambda d, n: ops.execReduceFloat(None, 1, A, info, None, B, row, d, n),
+             lambda d, n: ops.execIndexReduceFloat(None, 0, A, info, None, B, row, d, n),
+             lambda d, n: ops.execSummaryStatsFloat(None, 0, A, info, None, B, row, d, n, True),
+             lambda d, n: ops.execReduce3Float(None, 1, A, info, None, B, info, C, row, d, n),
+             lambda d, n: ops._execReduce3All(0, None, 1, A, info, None, B, info, C, info, d, n),
+             lambda d, n: ops.execBroadcastFloat(None, 0, A, info, B, row, C, info, d, n),
+             lambda d, n: ops.execChain(0, None, 0, A, info, B, row, d, n, 0, None, 0, None, None, None, C, info))
+    for call in calls:
+        with pytest.raises(native_ops.Nd4jError, match="dimension list holds 1 entries, not 4"):
+            call([1], 4)
