@@ -77,13 +77,21 @@ def _dims(a, n):
 
 
 def _descriptor(a):
-    """A shapeInfo (or another list of 64-bit integers) as the bytes that a C function reads, and as a list. (An array's
-    own address costs ctypes ten times as much.)"""
+    """A list of 64-bit integers as the bytes that a C function reads, and as a list. (An array's own address costs ctypes
+    ten times as much.)"""
     if a is None:
         return None, None
     if type(a) is not np.ndarray or a.dtype != np.int64:
         a = np.asarray(a, dtype=np.int64)
     return a.tobytes(), a.tolist()
+
+
+def _shape(a):
+    """_descriptor of a shapeInfo, which has to be as long as its rank says."""
+    p, a = _descriptor(a)
+    if a is not None and len(a) < (2 * a[0] + 4 if a else 1):
+        raise Nd4jError(1, "a shapeInfo holds %d entries, fewer than its rank asks for" % len(a))
+    return p, a
 
 
 def load_library(path=None):
@@ -482,8 +490,8 @@ class NativeOps:
         """z = (x - mean) * invStd * gain + bias for every TAD of x along `dimension` (nd4jb200_exec_layer_norm). gain,
         bias, mean and invStd may be None."""
         kind, wide, _ = self._kinds(dt)
-        xsp, xl = _descriptor(xShapeInfo)
-        zsp, zl = (xsp, xl) if zShapeInfo is xShapeInfo else _descriptor(zShapeInfo)
+        xsp, xl = _shape(xShapeInfo)
+        zsp, zl = (xsp, xl) if zShapeInfo is xShapeInfo else _shape(zShapeInfo)
         dims = self._axes(dimension, dimensionLength)
         count, length = self._tads(xl, dims)
         device = self.lib.nd4jb200_get_device()
@@ -497,9 +505,9 @@ class NativeOps:
                           dBias, dimension, dimensionLength):
         """Gradients of execLayerNorm (nd4jb200_exec_layer_norm_grad). gain, dx, dGain and dBias may be None."""
         kind, wide, _ = self._kinds(dt)
-        xsp, xl = _descriptor(xShapeInfo)
-        dsp, dl = (xsp, xl) if dzShapeInfo is xShapeInfo else _descriptor(dzShapeInfo)
-        osp, ol = (xsp, xl) if dxShapeInfo is xShapeInfo else _descriptor(dxShapeInfo)
+        xsp, xl = _shape(xShapeInfo)
+        dsp, dl = (xsp, xl) if dzShapeInfo is xShapeInfo else _shape(dzShapeInfo)
+        osp, ol = (xsp, xl) if dxShapeInfo is xShapeInfo else _shape(dxShapeInfo)
         dims = self._axes(dimension, dimensionLength)
         count, length = self._tads(xl, dims)
         device = self.lib.nd4jb200_get_device()
@@ -515,7 +523,7 @@ class NativeOps:
         """Log probabilities of `tokens` (int64 on the device, one per row) under the rows of the logits, their
         entropies, row statistics and k best entries (nd4jb200_exec_token_log_probs). Results may be None."""
         kind, wide, whole = self._kinds(dt)
-        xsp, xl = _descriptor(logitsShapeInfo)
+        xsp, xl = _shape(logitsShapeInfo)
         rows = xl[1]
         device = self.lib.nd4jb200_get_device()
         self._check(self.lib.nd4jb200_exec_token_log_probs(
@@ -530,8 +538,8 @@ class NativeOps:
         """Gradient of execTokenLogProbs' log probabilities and entropies (nd4jb200_exec_token_log_probs_grad);
         gLogProbs or gEntropy may be None."""
         kind, wide, whole = self._kinds(dt)
-        xsp, xl = _descriptor(logitsShapeInfo)
-        osp, ol = (xsp, xl) if dLogitsShapeInfo is logitsShapeInfo else _descriptor(dLogitsShapeInfo)
+        xsp, xl = _shape(logitsShapeInfo)
+        osp, ol = (xsp, xl) if dLogitsShapeInfo is logitsShapeInfo else _shape(dLogitsShapeInfo)
         rows = xl[1]
         device = self.lib.nd4jb200_get_device()
         self._check(self.lib.nd4jb200_exec_token_log_probs_grad(
@@ -544,8 +552,8 @@ class NativeOps:
     def execEmbedding(self, dt, extraPointers, table, tableShapeInfo, tokens, scale, z, zShapeInfo):
         """Row i of z = scale * row tokens[i] of the table (nd4jb200_exec_embedding)."""
         kind, _, whole = self._kinds(dt)
-        tsp, tl = _descriptor(tableShapeInfo)
-        zsp, zl = _descriptor(zShapeInfo)
+        tsp, tl = _shape(tableShapeInfo)
+        zsp, zl = _shape(zShapeInfo)
         device = self.lib.nd4jb200_get_device()
         self._check(self.lib.nd4jb200_exec_embedding(
             self._queue(extraPointers), dt, self._array(table, "table", device, kind, tl), tsp,
@@ -554,8 +562,8 @@ class NativeOps:
     def execEmbeddingGrad(self, dt, extraPointers, tokens, scale, dz, dzShapeInfo, grad, gradShapeInfo, accumulate=False):
         """Gradient of the table of execEmbedding (nd4jb200_exec_embedding_grad)."""
         kind, _, whole = self._kinds(dt)
-        dsp, dl = _descriptor(dzShapeInfo)
-        gsp, gl = _descriptor(gradShapeInfo)
+        dsp, dl = _shape(dzShapeInfo)
+        gsp, gl = _shape(gradShapeInfo)
         device = self.lib.nd4jb200_get_device()
         self._check(self.lib.nd4jb200_exec_embedding_grad(
             self._queue(extraPointers), dt, self._tensor(tokens, "tokens", device, whole, dl[1]), scale,

@@ -242,3 +242,21 @@ def test_the_other_members_do_not_read_beyond_a_dimension_list_either(lib):
     for call in calls:
         with pytest.raises(native_ops.Nd4jError, match="dimension list holds 1 entries, not 4"):
             call([1], 4)
+
+
+def test_the_mirror_does_not_read_beyond_a_descriptor(lib):
+    ops = native_ops.NativeOps()
+    good = S.shape_info([4, 8])
+    for bad in (good[:7], list(good[:3]), [], [32] + [1] * 60):
+        for call in (lambda: ops.execLayerNorm(0, None, A, bad, None, None, 1e-5, B, bad, None, None, [1], 1),
+                     lambda: ops.execLayerNorm(0, None, A, good, None, None, 1e-5, B, bad, None, None, [1], 1),
+                     lambda: ops.execLayerNormGrad(0, None, A, good, None, B, C, D, bad, E, good, None, None, [1], 1),
+                     lambda: ops.execLayerNormGrad(0, None, A, good, None, B, C, D, good, E, bad, None, None, [1], 1),
+                     lambda: ops.execTokenLogProbs(0, None, A, bad, B, 1.0, C, None, None, None),
+                     lambda: ops.execTokenLogProbsGrad(0, None, A, good, B, 1.0, C, D, None, E, None, F, bad),
+                     lambda: ops.execEmbedding(0, None, A, bad, B, 1.0, C, good),
+                     lambda: ops.execEmbedding(0, None, A, good, B, 1.0, C, bad),
+                     lambda: ops.execEmbeddingGrad(0, None, A, 1.0, B, bad, C, good),
+                     lambda: ops.execEmbeddingGrad(0, None, A, 1.0, B, good, C, bad)):
+            with pytest.raises(native_ops.Nd4jError, match="fewer than its rank"):
+                call()
