@@ -317,7 +317,7 @@ int nd4jb200_exec_meta_predicate_strided(void *stream, int dtype, int opTypeA, i
  * `stream` and nothing waits. "Wide" values (statistics, log probabilities, norms) are float for float and half data
  * and double for double; sums are held in that type and results rounded once. Vectors (gain, bias, per-row values) are
  * dense. A result may take the place of an operand where that is said, with the same address and layout; other overlaps
- * are refused where they can be seen. All of them can be captured into a graph; scratch memory belongs to the call.
+ * are refused where they can be seen, and so is a result two of whose elements share a place. All of them can be captured into a graph; scratch memory belongs to the call.
  *
  * exec_layer_norm: for every TAD of x along `dimension`, z = (x - mean) / sqrt(variance + epsilon) * gain + bias, the
  * variance being sum((x - mean)^2) / n. gain and bias hold one value per element of a TAD (c-order of its axes) and may

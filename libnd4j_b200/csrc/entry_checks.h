@@ -4,6 +4,7 @@
 #pragma once
 #include <cmath>
 #include <exception>
+#include <numeric>
 #include <sstream>
 #include "runtime.h"
 
@@ -113,10 +114,26 @@ inline Status check_apart(const Span &a, const char *aName, const Span &b, const
     if (a.filled && b.filled && meet(a, b)) return bad_arg(std::string(aName) + " overlaps " + bName);
     return kOk;
 }
-// A written array needs a place of its own for every element.
+// A written array needs a place of its own for every element: two of them would be written by different CTAs, in an order
+// that nothing fixes. Two axes of strides s and t meet where i s = j t, first at i = t / gcd, j = s / gcd; an array may not
+// reach that far along both (for matrices this is exact). And no array has more elements than its span has places.
 inline Status check_written(const ShapeDesc &d, const char *name) {
-    for (int i = 0; i < d.rank; i++)
-        if (d.shape[i] > 1 && d.stride[i] == 0) return bad_arg(std::string(name) + ": a result cannot have a stride of 0");
+    if (d.length < 2) return kOk;
+    unsigned long long reach = 0;
+    for (int i = 0; i < d.rank; i++) {
+        if (d.shape[i] < 2) continue;
+        if (d.stride[i] == 0) return bad_arg(std::string(name) + ": a result cannot have a stride of 0");
+        const unsigned long long s = d.stride[i] < 0 ? 0 - (unsigned long long) d.stride[i] : (unsigned long long) d.stride[i];
+        reach += s * (unsigned long long) (d.shape[i] - 1);
+        for (int j = 0; j < i; j++) {
+            if (d.shape[j] < 2) continue;
+            const unsigned long long t = d.stride[j] < 0 ? 0 - (unsigned long long) d.stride[j] : (unsigned long long) d.stride[j];
+            const unsigned long long g = std::gcd(s, t);
+            if (t / g < (unsigned long long) d.shape[i] && s / g < (unsigned long long) d.shape[j])
+                return bad_arg(std::string(name) + ": a result cannot have elements that share their place");
+        }
+    }
+    if (reach < (unsigned long long) (d.length - 1)) return bad_arg(std::string(name) + ": a result cannot have elements that share their place");
     return kOk;
 }
 inline bool equal_shape(const ShapeDesc &a, const ShapeDesc &b) {

@@ -260,3 +260,38 @@ def test_the_mirror_does_not_read_beyond_a_descriptor(lib):
                      lambda: ops.execEmbeddingGrad(0, None, A, 1.0, B, good, C, bad)):
             with pytest.raises(native_ops.Nd4jError, match="fewer than its rank"):
                 call()
+
+
+# layouts of results: whether two elements share a place is counted out
+SHARED = [((4, 8), (7, 1)), ((4, 8), (1, 3)), ((4, 8), (-7, 1)), ((4, 8), (1, 1)), ((4, 8), (6, 4)), ((2, 3, 4), (6, 4, 1)), ((3, 3, 3), (1, 2, 4)),
+          ((4, 1, 8), (5, 0, -1))]
+APART = [((4, 8), (8, 1)), ((4, 8), (9, 1)), ((4, 8), (1, 4)), ((4, 8), (16, 2)), ((3, 2), (2, 3)), ((2, 2), (3, 2)), ((1, 8), (0, 1)), ((8, 1), (1, 0)),
+         ((4, 8), (-8, -1)), ((2, 3, 4), (12, 4, 1)), ((2, 3, 4), (1, 2, 6)), ((7, 5), (5, 7))]
+
+
+def test_the_layouts_do_and_do_not_share_places():
+    for cases, want in ((SHARED, True), (APART, False)):
+        for shape, strides in cases:
+            places = [sum(i * s for i, s in zip(at, strides)) for at in np.ndindex(*shape)]
+            assert (len(set(places)) < len(places)) is want, (shape, strides)
+
+
+@pytest.mark.parametrize("shape,strides", SHARED)
+def test_results_whose_elements_share_their_place(lib, shape, strides):
+    last = ints([len(shape) - 1])
+    word = "share their place"
+    plain, odd = dense(*shape), strided(shape, strides)
+    refused(lib, lib.nd4jb200_exec_layer_norm(None, 0, A, plain, None, None, 1e-5, B, odd, None, None, last, 1), word)
+    refused(lib, lib.nd4jb200_exec_layer_norm(None, 0, A, odd, None, None, 1e-5, A, odd, None, None, last, 1), word)
+    refused(lib, lib.nd4jb200_exec_layer_norm_grad(None, 0, A, plain, None, B, C, D, plain, E, odd, None, None, last, 1), word)
+    if len(shape) == 2:
+        refused(lib, lib.nd4jb200_exec_token_log_probs_grad(None, 0, A, plain, B, 1.0, C, D, None, E, None, F, odd), word)
+        refused(lib, lib.nd4jb200_exec_embedding(None, 0, A, dense(100, shape[1]), B, 1.0, C, odd), word)
+        refused(lib, lib.nd4jb200_exec_embedding_grad(None, 0, B, 1.0, C, dense(5, shape[1]), A, odd, 1), word)
+
+
+@pytest.mark.parametrize("shape,strides", APART)
+def test_results_whose_elements_lie_apart(lib, shape, strides):
+    # the next check is reached: the statistics stand in the operand
+    rc = lib.nd4jb200_exec_layer_norm(None, 0, A, dense(*shape), None, None, 1e-5, B, strided(shape, strides), A, None, ints([len(shape) - 1]), 1)
+    refused(lib, rc, "mean overlaps")
