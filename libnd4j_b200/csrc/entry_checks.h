@@ -91,7 +91,15 @@ inline Span span_of(const void *p, LL n, size_t elem) {
     const uintptr_t base = reinterpret_cast<uintptr_t>(p);
     return Span{base, base + (uintptr_t) n * elem, true};
 }
-inline bool meet(const Span &a, const Span &b) { return a.lo < b.hi && b.lo < a.hi && a.lo < a.hi && b.lo < b.hi; }
+// Whether two arrays certainly share bytes. The first and the last byte of a span belong to an element in any case, and
+// those between to one where the span is filled.
+inline bool meet(const Span &a, const Span &b) {
+    if (!(a.lo < b.hi && b.lo < a.hi && a.lo < a.hi && b.lo < b.hi)) return false;
+    if (a.filled && b.filled) return true;
+    if (a.lo == b.lo || a.hi == b.hi) return true;
+    const bool inA = a.lo <= b.lo || b.hi <= a.hi, inB = b.lo <= a.lo || a.hi <= b.hi;     // an end of one inside the other
+    return (a.filled && inA) || (b.filled && inB);
+}
 
 inline bool same_layout(const ShapeDesc &a, const ShapeDesc &b) {
     if (a.rank != b.rank) return false;
@@ -106,12 +114,12 @@ inline Status check_alias(const void *out, const ShapeDesc &od, const char *outN
                           const char *inName, size_t elem) {
     if (out == in && same_layout(od, id)) return kOk;
     const Span a = span_of(out, od, elem), b = span_of(in, id, elem);
-    if (a.filled && b.filled && meet(a, b))
+    if (meet(a, b) || (out == in && od.length > 0))
         return bad_arg(std::string(outName) + " overlaps " + inName + " without being the same array");
     return kOk;
 }
 inline Status check_apart(const Span &a, const char *aName, const Span &b, const char *bName) {
-    if (a.filled && b.filled && meet(a, b)) return bad_arg(std::string(aName) + " overlaps " + bName);
+    if (meet(a, b)) return bad_arg(std::string(aName) + " overlaps " + bName);
     return kOk;
 }
 // A written array needs a place of its own for every element: two of them would be written by different CTAs, in an order

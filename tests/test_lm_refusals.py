@@ -295,3 +295,26 @@ def test_results_whose_elements_lie_apart(lib, shape, strides):
     # the next check is reached: the statistics stand in the operand
     rc = lib.nd4jb200_exec_layer_norm(None, 0, A, dense(*shape), None, None, 1e-5, B, strided(shape, strides), A, None, ints([len(shape) - 1]), 1)
     refused(lib, rc, "mean overlaps")
+
+
+def test_overlaps_of_arrays_with_gaps(lib):
+    # rows 80 floats apart, of which 64 are the array's: the first and the last element are known to be there
+    one, other = strided((8, 64), (80, 1)), strided((8, 64), (72, 1))
+
+    def norm(x=A, xi=one, gain=B, z=C, zi=one, mean=D, eps=1e-5):
+        return lib.nd4jb200_exec_layer_norm(None, 0, x, xi, gain, None, eps, z, zi, mean, None, ints([1]), 1)
+    refused(lib, norm(z=A, zi=other), "overlaps")                       # the same first element, other rows
+    refused(lib, norm(z=A, zi=strided((8, 64), (-80, 1))), "overlaps")  # ... in other directions
+    refused(lib, norm(z=A + 4 * 56, zi=other), "overlaps")              # the same last element
+    refused(lib, norm(z=A - 4 * 100, zi=dense(8, 64)), "overlaps")      # the first one inside a dense array
+    refused(lib, norm(z=A + 4 * 500, zi=dense(8, 64)), "overlaps")      # the last one
+    refused(lib, norm(mean=A), "overlaps")
+    refused(lib, norm(gain=C + 4 * (7 * 80 + 63)), "overlaps")          # its first value is z's last
+    # what may lie in the gaps is let through, up to a check behind these
+    beyond = dict(mean=D + 1)
+    refused(lib, norm(z=A + 4 * 64, zi=strided((8, 16), (80, 1)), xi=strided((8, 16), (80, 1)), **beyond), "aligned")
+    refused(lib, norm(x=A, xi=strided((8, 40), (80, 2)), z=A + 4, zi=strided((8, 40), (80, 2)), **beyond), "aligned")
+    rc = lib.nd4jb200_exec_token_log_probs_grad(None, 0, A, one, B, 1.0, C, D, None, E, None, A, other)
+    refused(lib, rc, "overlaps")
+    rc = lib.nd4jb200_exec_embedding_grad(None, 0, B, 1.0, A + 4 * (7 * 80 + 63), dense(5, 64), A, one, 0)
+    refused(lib, rc, "overlaps")
