@@ -316,8 +316,11 @@ int nd4jb200_exec_meta_predicate_strided(void *stream, int dtype, int opTypeA, i
  * device pointers of the call's element type, shapeInfo and dimension arrays are host arrays, everything is queued on
  * `stream` and nothing waits. "Wide" values (statistics, log probabilities, norms) are float for float and half data
  * and double for double; sums are held in that type and results rounded once. Vectors (gain, bias, per-row values) are
- * dense. A result may take the place of an operand where that is said, with the same address and layout; other overlaps
- * are refused where they can be seen, and so is a result two of whose elements share a place. All of them can be captured into a graph; scratch memory belongs to the call.
+ * dense. A result may take the place of an operand where that is said, with the same address and layout; other
+ * overlaps are refused where they can be seen, and so is a result two of whose elements share a place. All of them can
+ * be captured into a graph; scratch memory belongs to the call. Of that the library keeps up to 1 GB per device for
+ * the calls to come, what lies beyond is given back at the next synchronisation; release_scratch gives back to the
+ * current device all that no queued call uses.
  *
  * exec_layer_norm: for every TAD of x along `dimension`, z = (x - mean) / sqrt(variance + epsilon) * gain + bias, the
  * variance being sum((x - mean)^2) / n. gain and bias hold one value per element of a TAD (c-order of its axes) and may
@@ -325,6 +328,7 @@ int nd4jb200_exec_meta_predicate_strided(void *stream, int dtype, int opTypeA, i
  * exec_layer_norm_grad: from x, mean, invStd (as written by the former) and the gradient dz of z, the gradients dx of
  * x, dGain and dBias of gain and bias; each of the three may be NULL. dx may take the place of x or dz. Without TADs
  * dGain and dBias are zero. */
+int nd4jb200_release_scratch(void);
 int nd4jb200_exec_layer_norm(void *stream, int dtype, const void *x, const Nd4jLong *xShapeInfo, const void *gain,
                              const void *bias, double epsilon, void *z, const Nd4jLong *zShapeInfo, void *mean,
                              void *invStd, const int *dimension, int dimensionLength);

@@ -1,8 +1,10 @@
 // Device-environment members of the boundary that the exec* families do not need themselves but that callers
 // of the reference's CUDA build resolve from the same library: peer-access control
 // (blas/NativeOps.h:2047-2058; blas/cuda/NativeOps.cu:3854-3938) and the constant-memory staging area
-// (blas/NativeOps.h:1836-1846; blas/cuda/NativeOps.cu:87, 4793-4834).
+// (blas/NativeOps.h:1836-1846; blas/cuda/NativeOps.cu:87, 4793-4834). And the release of scratch memory, which has no
+// counterpart there.
 #include "../../include/nd4j_b200.h"
+#include "entry_checks.h"
 #include "runtime.h"
 
 using namespace nd4jb200;
@@ -83,6 +85,8 @@ void *nd4jb200_get_constant_space(void) {
     if (e != cudaSuccess) { cuda_fail(e, "cudaGetSymbolAddress(constant space)"); return nullptr; }
     return p;
 }
+
+int nd4jb200_release_scratch(void) { return c_entry([] { return release_scratch(); }); }
 
 }  // extern "C"
 #pragma GCC visibility pop

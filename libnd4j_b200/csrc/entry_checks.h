@@ -24,7 +24,11 @@ template <class F> inline int c_entry(F body) noexcept {
 // order. Unlike the per-stream workspace it is never shared: calls from several host threads on one stream, and
 // graphs captured on one stream and replayed on several, each work in memory of their own. (Inside a capture the
 // allocation becomes a node of the graph.) The pool keeps what it was given, so that an eager call costs about a
-// microsecond of host time.
+// microsecond of host time, up to kScratchKept bytes per device: what it holds beyond that goes back to the device at the
+// next synchronisation, and all that is not in use with nd4jb200_release_scratch. A table gradient over 32768 tokens of 2048
+// halves takes 9 MB, layer norm's weights over rows of 4096 floats 10; a call that has to map its memory anew pays for it
+// (512 MB: 1.6 ms with what it needs in the pool, 6.9 without).
+constexpr unsigned long long kScratchKept = 1ull << 30;
 class Scratch {
 public:
     explicit Scratch(cudaStream_t s) : stream(s) {}
@@ -37,6 +41,9 @@ private:
     cudaStream_t stream;
     void *ptr = nullptr;
 };
+// Gives back to the current device what its pool holds and no call uses.
+Status release_scratch();
+
 // Lets a kernel use `bytes` of dynamic shared memory, asked for once per kernel and device (about a microsecond each time
 // otherwise). `asked` is the kernel's own word, one bit per device.
 inline Status allow_shared(const void *kernel, size_t bytes, std::atomic<unsigned long long> &asked) {

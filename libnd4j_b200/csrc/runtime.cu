@@ -132,7 +132,7 @@ Status Scratch::alloc(size_t bytes) {
             props.location.type = cudaMemLocationTypeDevice;
             props.location.id = device;
             cudaError_t e = cudaMemPoolCreate(&pool, &props);
-            unsigned long long keep = ~0ull;
+            unsigned long long keep = kScratchKept;
             if (e == cudaSuccess) e = cudaMemPoolSetAttribute(pool, cudaMemPoolAttrReleaseThreshold, &keep);
             const cudaError_t back = cudaThreadExchangeStreamCaptureMode(&mode);
             if (e != cudaSuccess) return cuda_fail(e, "cudaMemPoolCreate(scratch)");
@@ -149,9 +149,17 @@ Status Scratch::alloc(size_t bytes) {
     return kOk;
 }
 
+Status release_scratch() {
+    int device = 0;
+    ND_CUDA(cudaGetDevice(&device));
+    std::lock_guard<std::mutex> lock(g_mu);
+    auto it = g_pools.find(device);
+    if (it != g_pools.end()) ND_CUDA(cudaMemPoolTrimTo(it->second, 0));
+    return kOk;
+}
+
 void release_workspaces() {
     std::lock_guard<std::mutex> lock(g_mu);
-    for (auto &kv : g_pools) cudaMemPoolTrimTo(kv.second, 0);
     for (auto &kv : g_blocks) {
         if (kv.second.dev) cudaFree(kv.second.dev);
         if (kv.second.host) cudaFreeHost(kv.second.host);

@@ -134,6 +134,7 @@ def load_library(path=None):
         "nd4jb200_exec_chain": (i, [vp, i, i, vp, llp, vp, llp, ip, i, i, vp, i, vp, llp, vp, vp, llp]),
         "nd4jb200_exec_meta_predicate_shape": (i, [vp, i, i, i, i, i, vp, llp, vp, llp, vp, llp, vp, vp, d, d]),
         "nd4jb200_exec_meta_predicate_strided": (i, [vp, i, i, i, i, i, ll, vp, ll, vp, ll, vp, ll, vp, vp, d, d]),
+        "nd4jb200_release_scratch": (i, []),
         "nd4jb200_exec_layer_norm": (i, [vp, i, vp, vp, vp, vp, d, vp, vp, vp, vp, vp, i]),
         "nd4jb200_exec_layer_norm_grad": (i, [vp, i, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, i]),
         "nd4jb200_exec_token_log_probs": (i, [vp, i, vp, vp, vp, d, vp, vp, vp, vp, i, vp, vp]),
@@ -484,6 +485,11 @@ class NativeOps:
             else:
                 count *= extent
         return count, length
+
+    def releaseScratch(self):
+        """Gives the scratch memory of these operators that no queued call uses back to the current device
+        (nd4jb200_release_scratch)."""
+        self._check(self.lib.nd4jb200_release_scratch())
 
     def execLayerNorm(self, dt, extraPointers, x, xShapeInfo, gain, bias, epsilon, z, zShapeInfo, mean, invStd, dimension,
                       dimensionLength):
