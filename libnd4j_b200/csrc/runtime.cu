@@ -31,9 +31,9 @@ namespace {
 struct Block { void *dev = nullptr; size_t cap = 0; void *host = nullptr; };
 std::mutex g_mu;
 std::map<std::pair<int, cudaStream_t>, Block> g_blocks;
-// Blocks that were outgrown. They stay allocated until release_workspaces(): a caller may have handed out
-// pointers into one (result slots, position lists) that launches still queued on the stream will use, and a
-// block grows by half each time, so everything retired together is smaller than twice the live block.
+// Blocks that were outgrown. They stay allocated: a caller may have handed out pointers into one (result slots,
+// position lists) that launches still queued on the stream, or captured into a graph, will use, and a block
+// grows by half each time, so everything retired together is smaller than twice the live block.
 std::vector<void *> g_retired;
 }  // namespace
 
@@ -156,23 +156,6 @@ Status release_scratch() {
     auto it = g_pools.find(device);
     if (it != g_pools.end()) ND_CUDA(cudaMemPoolTrimTo(it->second, 0));
     return kOk;
-}
-
-void release_workspaces() {
-    std::lock_guard<std::mutex> lock(g_mu);
-    for (auto &kv : g_blocks) {
-        if (kv.second.dev) cudaFree(kv.second.dev);
-        if (kv.second.host) cudaFreeHost(kv.second.host);
-    }
-    g_blocks.clear();
-    for (void *p : g_retired) cudaFree(p);
-    g_retired.clear();
-    for (auto &kv : g_staging)
-        for (int k = 0; k < 4; k++) {
-            if (kv.second.buf[k]) cudaFreeHost(kv.second.buf[k]);
-            if (kv.second.done[k]) cudaEventDestroy(kv.second.done[k]);
-        }
-    g_staging.clear();
 }
 
 }  // namespace nd4jb200

@@ -23,15 +23,14 @@ Status cuda_fail(cudaError_t e, const char *where);
     } while (0)
 
 // Scratch memory owned by the library, one block per (device, stream) so that calls on
-// different streams never share it. The block only ever grows; an outgrown block is kept until
-// release_workspaces(), so pointers into it stay valid for work already queued.
+// different streams never share it. The block only ever grows; an outgrown block is kept, so
+// pointers into it stay valid for work already queued.
 // `hostSlot`, when requested, is a 64-byte pinned buffer used to bring scalar results back.
 Status workspace(cudaStream_t stream, size_t bytes, void **dev, void **hostSlot);
 // Layout of a workspace block: [256-byte result slot][kCounterSlots arrival counters, always left zero]
 // [scratch: partial states, index lists]. Only the part from kWorkspaceScratch on is free for a call to use.
 constexpr size_t kCounterSlots = 65536;
 constexpr size_t kWorkspaceScratch = 256 + kCounterSlots * sizeof(unsigned);
-void release_workspaces();
 
 // Host-to-device copy of a small list (pointer tables, swap lists) that does not stall the caller: the bytes are
 // copied into a pinned staging buffer owned by the library (a ring of four per device and stream, each guarded by
