@@ -355,9 +355,10 @@ int nd4jb200_exec_token_log_probs_grad(void *stream, int dtype, const void *logi
                                        const Nd4jLong *dLogitsShapeInfo);
 /* exec_embedding: row i of z = scale * row tokens[i] of the table (both rank 2, tokens on the device, one per row of
  * z). A negative token gives a row of zeros, one at or beyond the table's end a row of NaN.
- * exec_embedding_grad: row v of grad = scale * the sum, in the order of i, of the rows i of dz with tokens[i] = v, added
- * to what grad holds when `accumulate` is not 0 (rows without a token are then left as they are), in place of it
- * otherwise (and zero in rows without a token). Tokens outside the table take no part. */
+ * exec_embedding_grad: row v of grad = scale * the sum of the rows i of dz with tokens[i] = v, added to what grad holds
+ * when `accumulate` is not 0 (rows without a token are then left as they are), in place of it otherwise (and zero in
+ * rows without a token). Tokens outside the table take no part. Rows are added in an order that the call's sizes, layouts
+ * and tokens fix: the same call gives the same bits. */
 int nd4jb200_exec_embedding(void *stream, int dtype, const void *table, const Nd4jLong *tableShapeInfo,
                             const Nd4jLong *tokens, double scale, void *z, const Nd4jLong *zShapeInfo);
 int nd4jb200_exec_embedding_grad(void *stream, int dtype, const Nd4jLong *tokens, double scale, const void *dz,

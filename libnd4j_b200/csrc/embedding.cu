@@ -10,8 +10,9 @@
 // commonest) would queue up on a few addresses. So the (token, position) pairs are sorted first, stably, which puts the
 // rows of a token next to each other in the order of their positions; the sorted list is cut into chunks of equal
 // length, a group of threads walks a chunk and writes every run that ends inside it, and a run that crosses a chunk's
-// end leaves partial sums, which a last launch folds in order. The result is the same bits on every run. Sums are held
-// in float (double for double data) and rounded once, after scaling and, where asked for, adding what grad holds.
+// end leaves partial sums, one for each chunk, which a last launch adds up: every eighth of them, then the eight sums.
+// That order follows from the sizes, the layouts and the tokens alone, so the result is the same bits on every run. Sums
+// are held in float (double for double data) and rounded once, after scaling and, where asked for, adding what grad holds.
 //
 // The sort is a least-significant-digit radix sort with digits of up to 9 bits: two passes up to a table of 2^18 rows.
 // Up to 65536 tokens one cluster of CTAs does all passes in one launch, the counts and the keys travelling through
@@ -429,7 +430,7 @@ __global__ void __launch_bounds__(kEmbThreads, 4) k_embedding_sums(const EmbArgs
 }
 
 // Runs that cross chunks: the CTA of the chunk that such a run begins in adds up the tail there and the heads of the
-// chunks it reaches, eight at a time, the eight sums in order. Most chunks have no such run and their CTA ends at once.
+// chunks it reaches, warp w every eighth of them, then the warps' eight sums. Most chunks have no such run and their CTA ends at once.
 template <class T>
 __global__ void __launch_bounds__(256) k_embedding_join(const EmbArgs a) {
     grid_dependency_sync();
