@@ -313,21 +313,21 @@ int nd4jb200_exec_meta_predicate_strided(void *stream, int dtype, int opTypeA, i
 
 /* ---- between a language model's matrix products ------------------------------------------------------------------
  * Operators without a counterpart among the reference's members, in the manner of the ones above: data pointers are
- * device pointers of the call's element type, shapeInfo and dimension arrays are host arrays, everything is queued on
- * `stream` and nothing waits. "Wide" values (statistics, log probabilities, norms) are float for float and half data
- * and double for double; sums are held in that type and results rounded once. Vectors (gain, bias, per-row values) are
- * dense. A result may take the place of an operand where that is said, with the same address and layout; other
- * overlaps are refused where they can be seen, and so is a result two of whose elements share a place. All of them can
- * be captured into a graph; scratch memory belongs to the call. Of that the library keeps up to 1 GB per device for
- * the calls to come, what lies beyond is given back at the next synchronisation; release_scratch gives back to the
- * current device all that no queued call uses.
+ * device pointers of the call's element type, shapeInfo and dimension arrays are host arrays, everything is queued
+ * on `stream` and nothing waits. "Wide" values (statistics, log probabilities, norms) are float for float and half
+ * data and double for double; sums (over rows too: dGain, dBias, a table's gradient) are held in that type and
+ * results rounded once. Vectors (gain, bias, per-row values) are dense. A result may take the place of an operand
+ * where that is said, with the same address and layout; other overlaps are refused where they can be seen, and so is
+ * a result two of whose elements share a place. All of them can be captured into a graph; scratch memory belongs to
+ * the call. Of that the library keeps up to 1 GB per device for the calls to come, what lies beyond is given back at
+ * the next synchronisation; release_scratch gives back to the current device all that no queued call uses.
  *
- * exec_layer_norm: for every TAD of x along `dimension`, z = (x - mean) / sqrt(variance + epsilon) * gain + bias, the
- * variance being sum((x - mean)^2) / n. gain and bias hold one value per element of a TAD (c-order of its axes) and may
- * be NULL (1 and 0); mean and invStd receive one wide value per TAD or are NULL. z may take x's place.
- * exec_layer_norm_grad: from x, mean, invStd (as written by the former) and the gradient dz of z, the gradients dx of
- * x, dGain and dBias of gain and bias; each of the three may be NULL. dx may take the place of x or dz. Without TADs
- * dGain and dBias are zero. */
+ * exec_layer_norm: for every TAD of x along `dimension`, z = (x - mean) / sqrt(variance + epsilon) * gain + bias,
+ * the variance being sum((x - mean)^2) / n. gain and bias hold one value per element of a TAD (c-order of its axes)
+ * and may be NULL (1 and 0); mean and invStd receive one wide value per TAD or are NULL. z may take x's place.
+ * exec_layer_norm_grad: from x, mean, invStd (as written by the former) and the gradient dz of z, the gradients dx
+ * of x, dGain and dBias of gain and bias; each of the three may be NULL. dx may take the place of x or dz. Without
+ * TADs dGain and dBias are zero. An x without elements leaves everything else as it is. */
 int nd4jb200_release_scratch(void);
 int nd4jb200_exec_layer_norm(void *stream, int dtype, const void *x, const Nd4jLong *xShapeInfo, const void *gain,
                              const void *bias, double epsilon, void *z, const Nd4jLong *zShapeInfo, void *mean,
@@ -338,14 +338,16 @@ int nd4jb200_exec_layer_norm_grad(void *stream, int dtype, const void *x, const 
                                   int dimensionLength);
 /* exec_token_log_probs: for every row x of the rank-2 logits, with p = softmax(scale * x): logProbs = log p[token],
  * entropy = -sum p log p, rowMax = max x, logSum = log sum exp(scale * (x - rowMax)), and the k best entries (larger
- * first, equal ones by index; a NaN before all) with their log probabilities, [rows, k] dense. k is at most 64 and at
- * most the row's length (0: topTokens and topLogProbs may be NULL); scale is positive. Each of the four per-row results may
- * be NULL; tokens (device, one per row) may be NULL when logProbs is. A negative token marks padding: its row is not read and gives zeros and best tokens of -1. A
- * token at or beyond the row's length gives a NaN. Entries of -inf have probability 0; a row of nothing else gives log
- * probability -inf and entropy 0, a row with a NaN or +inf gives NaN.
+ * first, equal ones by index; a NaN before all) with their log probabilities, [rows, k] dense. k is at most 64 and
+ * at most the row's length (0: topTokens and topLogProbs may be NULL); scale is positive and at most 1e30. Each of
+ * the four per-row results may be NULL; tokens (device, one per row) may be NULL when logProbs is. A negative token
+ * marks padding: its row does not count, whatever it holds, and gives zeros and best tokens of -1. A token at or
+ * beyond the row's length gives a NaN. Entries of -inf have probability 0; a row of nothing else gives log
+ * probability -inf and entropy 0, a row with a NaN or +inf gives NaN. Exponentials of float and half data are off by
+ * up to 2^-22 relative.
  * exec_token_log_probs_grad: dLogits of  sum gLogProbs * logProbs + gEntropy * entropy  (one of the two may be NULL;
- * entropy is needed for the second), from the values the former wrote. Rows of padding, and of -inf alone, get zeros; a
- * token at or beyond the row's length a row of NaN. dLogits may take the place of the logits. */
+ * entropy is needed for the second), from the values the former wrote. Rows of padding, and of -inf alone, get
+ * zeros, but a token at or beyond the row's length a row of NaN. dLogits may take the place of the logits. */
 int nd4jb200_exec_token_log_probs(void *stream, int dtype, const void *logits, const Nd4jLong *logitsShapeInfo,
                                   const Nd4jLong *tokens, double scale, void *logProbs, void *entropy, void *rowMax,
                                   void *logSum, int k, Nd4jLong *topTokens, void *topLogProbs);
@@ -355,19 +357,20 @@ int nd4jb200_exec_token_log_probs_grad(void *stream, int dtype, const void *logi
                                        const Nd4jLong *dLogitsShapeInfo);
 /* exec_embedding: row i of z = scale * row tokens[i] of the table (both rank 2, tokens on the device, one per row of
  * z). A negative token gives a row of zeros, one at or beyond the table's end a row of NaN.
- * exec_embedding_grad: row v of grad = scale * the sum of the rows i of dz with tokens[i] = v, added to what grad holds
- * when `accumulate` is not 0 (rows without a token are then left as they are), in place of it otherwise (and zero in
- * rows without a token). Tokens outside the table take no part. Rows are added in an order that the call's sizes, layouts
- * and tokens fix: the same call gives the same bits. */
+ * exec_embedding_grad: row v of grad = scale * the sum of the rows i of dz with tokens[i] = v, added to what grad
+ * holds when `accumulate` is not 0 (rows without a token are then left as they are), in place of it otherwise (and
+ * zero in rows without a token). Tokens outside the table take no part. Rows are added in an order that the call's
+ * sizes, layouts, alignment and tokens fix: the same call gives the same bits. */
 int nd4jb200_exec_embedding(void *stream, int dtype, const void *table, const Nd4jLong *tableShapeInfo,
                             const Nd4jLong *tokens, double scale, void *z, const Nd4jLong *zShapeInfo);
 int nd4jb200_exec_embedding_grad(void *stream, int dtype, const Nd4jLong *tokens, double scale, const void *dz,
                                  const Nd4jLong *dzShapeInfo, void *grad, const Nd4jLong *gradShapeInfo, int accumulate);
-/* exec_global_norm: norm (device, one wide value) = the square root of the sum of the squares of all values of n dense
- * tensors. `x` and `lengths` are host arrays, as for average / accumulate; a tensor of length 0 may be NULL.
+/* exec_global_norm: norm (device, one wide value) = the square root of the sum of the squares of all values of n
+ * dense tensors. `x` and `lengths` are host arrays, as for average / accumulate; a tensor of length 0 may be NULL.
  * exec_clip_by_global_norm: writes the norm and, tensor by tensor, z = x * min(1, maxNorm / norm) (z == NULL: in
  * place; z[i] may be x[i]). A norm that is not finite as a wide value scales nothing: z = x. No result may overlap
- * another tensor's memory. */
+ * another tensor's memory. Squares are added in double, so doubles beyond 1.3e154 have an infinite norm and those
+ * below 1e-162 count as 0. */
 int nd4jb200_exec_global_norm(void *stream, int dtype, const void *const *x, const Nd4jLong *lengths, int n, void *norm);
 int nd4jb200_exec_clip_by_global_norm(void *stream, int dtype, const void *const *x, void *const *z,
                                       const Nd4jLong *lengths, int n, double maxNorm, void *norm);

@@ -9,7 +9,8 @@
 // more sweeps. Here a row is read once, as fast as HBM delivers it, each thread carrying the running maximum of what it
 // has seen and the two sums relative to it, rescaled in the rare step that moves the maximum; nothing but the results
 // is written. Sums are held in float for float and half data, in double for double. Measured: 4096 rows of 32768 floats,
-// 84 us = 6.4 TB/s (HBM); 8192 rows of 50001 halves, 147 us = 5.6 TB/s (HBM and, at 0.7, the exponentials).
+// 82 us = 6.5 TB/s a call among others, 94 with cold caches (HBM); 8192 rows of 50001 halves with entropy, 154 us = 5.3
+// TB/s with cold caches (HBM and, at 0.7, the exponentials).
 //
 // Exponentials are powers of two (one special-function instruction, relative error 2^-22), so c carries the factor log2(e).
 // Half data: the distance from the reference point is one fused multiply-add, x c - R. R is the rounded m c; every term is
@@ -564,7 +565,7 @@ __global__ void __launch_bounds__(LT, lp_ctas<T>(LT)) k_token_log_probs(const Lp
 // Reads a word, writes a word. What costs beside the traffic is the wait for a row's values before anything can be
 // computed, so small CTAs, many per SM, each with all its words in flight from the start (8192 rows of 50001 halves: 291 us
 // with 256 threads of 4 words that waited for the row's values first, 277 so; 4096 rows of 32768 floats with entropy:
-// 182, 176).
+// 182, 170).
 constexpr int kLpGradThreads = 128;
 template <class T> constexpr int kLpGradWords = sizeof(T) == 2 ? 8 : 4;       // per thread
 template <class T> constexpr int kLpGradCtas = sizeof(T) == 2 ? 8 : 10;
@@ -650,7 +651,9 @@ template <class K> void launch_log_probs(K kernel, const LpArgs &a, unsigned gri
     count_launch();
 }
 
-// Half data leaves the fused form once the rounding of the largest 65504 c exceeds half an exponent (scale above 177).
+// Half data leaves the fused form once the rounding of the largest 65504 c exceeds half an exponent (scale above 177). The
+// other form takes an instruction more per element: 8192 rows of 50001 halves, 160 us against 154; their gradient 326
+// against 279.
 bool lp_far(const LpArgs &a) { return a.scale * LpMath<__half>::kUnit * 65504.0 > 16777216.0; }
 
 template <class T, int V, int LT, bool FAR> void lp_forward_kernels(const LpArgs &a, unsigned grid, cudaStream_t st) {
