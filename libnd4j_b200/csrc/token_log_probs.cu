@@ -564,8 +564,8 @@ __global__ void __launch_bounds__(LT, lp_ctas<T>(LT)) k_token_log_probs(const Lp
 // ---- gradient ----------------------------------------------------------------------------------------------------
 // Reads a word, writes a word. What costs beside the traffic is the wait for a row's values before anything can be
 // computed, so small CTAs, many per SM, each with all its words in flight from the start (8192 rows of 50001 halves: 291 us
-// with 256 threads of 4 words that waited for the row's values first, 277 so; 4096 rows of 32768 floats with entropy:
-// 182, 170).
+// with 256 threads of 4 words that waited for the row's values first, 272 so, 307 where the maximum is loaded only for
+// tokens inside the row; 4096 rows of 32768 floats with entropy: 182, 168).
 constexpr int kLpGradThreads = 128;
 template <class T> constexpr int kLpGradWords = sizeof(T) == 2 ? 8 : 4;       // per thread
 template <class T> constexpr int kLpGradCtas = sizeof(T) == 2 ? 8 : 10;
@@ -590,15 +590,16 @@ __global__ void __launch_bounds__(kLpGradThreads, kLpGradCtas<T>) k_token_log_pr
         for (int j = 0; j < W; j++)
             if (first + j * kLpGradThreads < row.words) row.load(first + j * kLpGradThreads, v[j]);
         const LL token = a.tokens[r];
-        const C m = static_cast<const C *>(a.rowMax)[r], logSum = static_cast<const C *>(a.logSum)[r];
+        C m = static_cast<const C *>(a.rowMax)[r];                // loaded for any token: it must not wait for that one
+        const C logSum = static_cast<const C *>(a.logSum)[r];
         const C g = (C) a.scale * (a.gLogProbs ? static_cast<const C *>(a.gLogProbs)[r] : C(0));
         const C h = ENT ? (C) a.scale * static_cast<const C *>(a.gEntropy)[r] : C(0);
-        // padding, or a row without a value: zeros; a token beyond the row stays visible there too
-        const bool none = token < 0 || (m == -C(INFINITY) && token < a.vocab);
+        if (token >= a.vocab) m = (C) NAN;                        // a row of NaN of any row, as where it holds a NaN
+        const bool none = token < 0 || m == -C(INFINITY);         // padding, or a row without a value: zeros
         const C ref = M::ref(m, c), shift = logSum * unit - M::off(m, ref, c);
         C A = ENT ? -(g + h * static_cast<const C *>(a.entropy)[r]) : -g;
         const C B = ENT ? -h * back : C(0);
-        if (token >= a.vocab || m != m) A = (C) NAN;
+        if (m != m) A = (C) NAN;
         auto one = [&](C x) -> C {
             const C lp = M::dist(x, ref, c) - shift, p = lp_exp(lp);
             return ENT ? p * fma(B, lp_finite(lp), A) : p * A;
@@ -652,8 +653,8 @@ template <class K> void launch_log_probs(K kernel, const LpArgs &a, unsigned gri
 }
 
 // Half data leaves the fused form once the rounding of the largest 65504 c exceeds half an exponent (scale above 177). The
-// other form takes an instruction more per element: 8192 rows of 50001 halves, 160 us against 154; their gradient 326
-// against 279.
+// other form takes an instruction more per element: 8192 rows of 50001 halves, 160 us against 154; their gradient 324
+// against 272.
 bool lp_far(const LpArgs &a) { return a.scale * LpMath<__half>::kUnit * 65504.0 > 16777216.0; }
 
 template <class T, int V, int LT, bool FAR> void lp_forward_kernels(const LpArgs &a, unsigned grid, cudaStream_t st) {
