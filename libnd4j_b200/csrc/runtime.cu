@@ -154,7 +154,14 @@ Status release_scratch() {
     ND_CUDA(cudaGetDevice(&device));
     std::lock_guard<std::mutex> lock(g_mu);
     auto it = g_pools.find(device);
-    if (it != g_pools.end()) ND_CUDA(cudaMemPoolTrimTo(it->second, 0));
+    if (it == g_pools.end()) return kOk;
+    // what is given back is in no queued call and no graph: it is allowed while a stream is captured
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    ND_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
+    const cudaError_t e = cudaMemPoolTrimTo(it->second, 0);
+    const cudaError_t back = cudaThreadExchangeStreamCaptureMode(&mode);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaMemPoolTrimTo(scratch)");
+    ND_CUDA(back);
     return kOk;
 }
 

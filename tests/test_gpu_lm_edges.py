@@ -255,3 +255,28 @@ def test_scratch_memory_goes_back_to_the_device(ops):
     ops.releaseScratch()
     held = free - torch.cuda.mem_get_info()[0]
     assert held <= 32 << 20, "%d MB are held after the release" % (held >> 20)
+
+
+def test_scratch_memory_is_released_while_a_stream_is_captured(ops):
+    x, dz = randn(1, 900, 512).float(), randn(2, 900, 512).float()
+    mean, inv = x.mean(1), 1 / torch.sqrt(x.var(1, correction=0) + 1e-5)
+    dx, dg = torch.empty_like(x), torch.empty(512, device="cuda")
+
+    def step(extra):
+        ops.execLayerNormGrad(0, extra, x, info(x), None, mean, inv, dz, info(dz), dx, info(dx), dg, None, [1], 1)
+    step(None)
+    torch.cuda.synchronize()
+    want = dx.clone(), dg.clone()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        extra = [None, torch.cuda.current_stream().cuda_stream]
+        step(extra)
+        ops.releaseScratch()
+        step(extra)
+    for t in (dx, dg):
+        t.fill_(9)
+    ops.releaseScratch()
+    g.replay()
+    step(None)
+    torch.cuda.synchronize()
+    assert torch.equal(dx, want[0]) and torch.equal(dg, want[1])
